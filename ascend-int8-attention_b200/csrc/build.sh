@@ -9,5 +9,5 @@ NVCC=${NVCC:-/usr/local/cuda/bin/nvcc}
     -Xcompiler -fPIC -Xcompiler -fvisibility=hidden \
     -shared -o "$out/libsharedkv_cuda.so" \
     "$here/c_abi.cu" "$here/cache_write.cu" "$here/decode_attention.cu" \
-    "$here/attention_static_scratch.cu"
+    "$here/attention_static_scratch.cu" "$here/tree_attention.cu" "$here/page_pool.cu"
 echo "built $out/libsharedkv_cuda.so"

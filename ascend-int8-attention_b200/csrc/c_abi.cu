@@ -10,6 +10,8 @@
 
 static_assert(sizeof(SharedKVArgs) == 200, "SharedKVArgs must stay 200 bytes");
 static_assert(sizeof(CacheWriteArgs) == 88, "CacheWriteArgs must stay 88 bytes");
+static_assert(sizeof(TreeAttentionArgs) == 192, "TreeAttentionArgs is mirrored by the Python layer");
+static_assert(sizeof(PagePoolArgs) == 64, "PagePoolArgs is mirrored by the Python layer");
 
 namespace sharedkv {
 
@@ -138,6 +140,61 @@ int sharedkv_attention_debug(uint32_t variant, void *stream, const SharedKVArgs 
 {
     if (!debug) return SHAREDKV_EINVAL;
     return sharedkv::attention(variant, args, static_cast<cudaStream_t>(stream), debug);
+}
+
+uint32_t sharedkv_tree_args_size(void) { return (uint32_t)sizeof(TreeAttentionArgs); }
+uint64_t sharedkv_tree_workspace_bytes(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk)
+{
+    return sharedkv::tree_workspace_bytes(tokens, heads, batch, ratio, topk);
+}
+int launch_tree_attention(void *stream, const TreeAttentionArgs *args)
+{
+    return sharedkv::tree_attention(args, static_cast<cudaStream_t>(stream));
+}
+int sharedkv_tree_attention(uint64_t args, int32_t device, void *stream)
+{
+    if (!args) return SHAREDKV_EINVAL;
+    sharedkv::DeviceScope scope(device);
+    if (scope.error != cudaSuccess) return (int)scope.error;
+    return sharedkv::tree_attention(reinterpret_cast<const TreeAttentionArgs *>(args), static_cast<cudaStream_t>(stream));
+}
+
+uint32_t sharedkv_page_args_size(void) { return (uint32_t)sizeof(PagePoolArgs); }
+uint64_t sharedkv_page_workspace_bytes(uint32_t batch, uint32_t width) { return sharedkv::page_workspace_bytes(batch, width); }
+int launch_page_resize(void *stream, const PagePoolArgs *args, const int32_t *wanted)
+{
+    return sharedkv::page_plan(0, args, wanted, static_cast<cudaStream_t>(stream));
+}
+int launch_page_fork(void *stream, const PagePoolArgs *args, const int32_t *parents)
+{
+    return sharedkv::page_plan(1, args, parents, static_cast<cudaStream_t>(stream));
+}
+int launch_page_copy(void *stream, const PagePoolArgs *args, const int32_t *pairs, uint32_t count)
+{
+    return sharedkv::page_copy(args, pairs, count, static_cast<cudaStream_t>(stream));
+}
+int launch_page_keep(void *stream, const PagePoolArgs *args, const int32_t *base, const int32_t *kept, uint32_t kept_width)
+{
+    return sharedkv::page_keep(args, base, kept, kept_width, static_cast<cudaStream_t>(stream));
+}
+int sharedkv_page(uint64_t args, uint32_t op, uint64_t a, uint64_t b, uint32_t n, int32_t device, void *stream)
+{
+    if (!args) return SHAREDKV_EINVAL;
+    sharedkv::DeviceScope scope(device);
+    if (scope.error != cudaSuccess) return (int)scope.error;
+    const PagePoolArgs *pool = reinterpret_cast<const PagePoolArgs *>(args);
+    const int32_t *first = reinterpret_cast<const int32_t *>(a), *second = reinterpret_cast<const int32_t *>(b);
+    switch (op) {
+        case 0: return launch_page_resize(stream, pool, first);
+        case 1: return launch_page_fork(stream, pool, first);
+        case 2: return launch_page_copy(stream, pool, first, n);
+        case 3: return launch_page_keep(stream, pool, first, second, n);
+        default: return SHAREDKV_EVARIANT;
+    }
+}
+int sharedkv_page_status(const void *workspace, void *stream)
+{
+    return sharedkv::page_status(workspace, static_cast<cudaStream_t>(stream));
 }
 
 const char *sharedkv_status_string(int status)

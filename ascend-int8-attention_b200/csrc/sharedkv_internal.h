@@ -56,4 +56,15 @@ int attention(uint32_t variant, const SharedKVArgs *args, cudaStream_t stream, c
 // SHAREDKV_ETIMEDOUT, or the cudaError_t of the read itself.
 int workspace_status(const void *workspace, cudaStream_t stream);
 
+// Drafted-tree attention (tree_attention.cu).
+uint64_t tree_workspace_bytes(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk);
+int tree_attention(const TreeAttentionArgs *args, cudaStream_t stream);
+
+// Page pool (page_pool.cu).  `op` 0 resizes to `input`, 1 forks from the parents `input`.
+uint64_t page_workspace_bytes(uint32_t batch, uint32_t width);
+int page_plan(uint32_t op, const PagePoolArgs *args, const int32_t *input, cudaStream_t stream);
+int page_copy(const PagePoolArgs *args, const int32_t *pairs, uint32_t count, cudaStream_t stream);
+int page_keep(const PagePoolArgs *args, const int32_t *base, const int32_t *kept, uint32_t kept_width, cudaStream_t stream);
+int page_status(const void *workspace, cudaStream_t stream);
+
 }  // namespace sharedkv

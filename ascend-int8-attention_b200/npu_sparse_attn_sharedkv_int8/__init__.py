@@ -1,8 +1,9 @@
 """INT8 shared-KV decode attention and paged INT8 KV-cache writer for NVIDIA B200.
 
 The import surface is that of the Ascend package of the same name
-(npu_sparse_attn_sharedkv_int8/__init__.py:7-23 of the reference): four public names, looked up
-on first use so that the data classes can be imported on a machine without CUDA.
+(npu_sparse_attn_sharedkv_int8/__init__.py:7-23 of the reference), four public names, and two of this
+build's own: drafted-tree attention and the page pool.  All are looked up on first use so that the
+data classes can be imported on a machine without CUDA.
 """
 import importlib
 
@@ -15,6 +16,8 @@ _HOME = {
     "SharedKVCase": "reference",
     "PreparedAttention": "attention",
     "PreparedCacheWrite": "cache",
+    "PreparedTreeAttention": "tree_attention",
+    "PagePool": "pages",
 }
 __all__ = sorted(_HOME)
 

@@ -247,6 +247,94 @@ SHAREDKV_API const char *sharedkv_status_string(int status);
 SHAREDKV_API int sharedkv_attention_static_scratch(uint32_t variant, void *stream, const SharedKVArgs *args);
 SHAREDKV_API int sharedkv_static_scratch_status(void *stream);
 
+/* ------------------------------------------------------------------ drafted trees
+ * Attention of a tree of drafted tokens over the INT8 shared-KV cache (speculative decoding): the
+ * tokens of a request are the nodes of a draft tree, and a token attends the committed rows and the
+ * rows of its own path instead of everything in front of it.  The reference has no such operator (its
+ * query tokens are one run, reference.py:224-253); types, page rules and padding rules are those of
+ * the attention entries above.
+ *
+ * Request b has n = cuQ[b+1] - cuQ[b] tokens and prefix = seqLens[b] - n committed rows; its token j
+ * owns logical row prefix + j of the original cache.  A token with path mask M (bit j: drafted row j
+ * of its request, itself included as a rule; bits >= n are ignored) and c = popcount(M) attends
+ *   - the committed rows prefix - (window - c) .. prefix - 1, as far as they exist,
+ *   - the drafted rows of its mask,
+ *   - ratio 128: compressed rows 0 .. prefix / 128 - 1 and, for every bit e of its cmpPaths mask,
+ *     row prefix / 128 + e (rows of groups that drafted tokens complete),
+ *   - ratio 4: every entry of its top-k list in [0, prefix / 4 + 64); an entry named twice counts twice.
+ * Rows beyond the block table, on a negative page id or on one outside the cache are no keys.  A token
+ * without any key gives zeros and LSE = sink; a sink of -inf is no sink.  Rows of `out` behind the last
+ * live token are written as zeros (LSE 0).  A query row that holds a NaN or an infinity gives NaN. */
+typedef struct TreeAttentionArgs {
+    uint64_t q;          /* BF16 [tokens, heads, 512], contiguous                        */
+    uint64_t ori;        /* INT8 original cache [oriPages, 32, 1, 512]                   */
+    uint64_t cmp;        /* INT8 compressed cache [cmpPages, 32, 1, 512] (ratio > 1)     */
+    uint64_t oriScale, cmpScale;      /* FP32 [512]                                      */
+    uint64_t oriTable, cmpTable;      /* INT32 [batch, width]                            */
+    uint64_t indices;    /* INT32 [tokens, 1, topk] (ratio 4 only)                       */
+    uint64_t paths;      /* INT64 [tokens] path masks                                    */
+    uint64_t cmpPaths;   /* INT64 [tokens] or 0 (ratio 128 only)                         */
+    uint64_t cuQ, seqLens;            /* INT32 [batch + 1], [batch]                      */
+    uint64_t sinks;      /* FP32 [heads]                                                 */
+    uint64_t out;        /* BF16 [tokens, heads, 512]                                    */
+    uint64_t lse;        /* FP32 [tokens, heads] or 0                                    */
+    uint64_t workspace;  /* >= sharedkv_tree_workspace_bytes(...) bytes, 256-aligned; needs no
+                            clearing; launches that can overlap need one each            */
+    uint64_t oriStride, cmpStride;    /* bytes between pages, multiples of 16            */
+    uint32_t tokens, heads, batch, oriTableWidth, cmpTableWidth, oriPages, cmpPages, ratio, window, topk;
+    float softmaxScale;
+    uint32_t reserved;
+} TreeAttentionArgs;
+SHAREDKV_API uint32_t sharedkv_tree_args_size(void);
+/* Scratch of one launch, in bytes.  `heads` is a multiple of 8 up to 128. */
+SHAREDKV_API uint64_t sharedkv_tree_workspace_bytes(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk);
+SHAREDKV_API int launch_tree_attention(void *stream, const TreeAttentionArgs *args);
+SHAREDKV_API int sharedkv_tree_attention(uint64_t args, int32_t device, void *stream);
+
+/* ------------------------------------------------------------------ page pool
+ * Page bookkeeping on the device, so that a captured decode loop needs no host round trip: a pool is
+ * a block table, sequence lengths, a reference count per page and the INT8 caches (one per layer)
+ * that share this page numbering.  A page is free when its count is zero; fresh pages are always the
+ * lowest-numbered free ones, so results do not depend on timing.  Sequence b holds the pages
+ * table[b, 0 .. ceil(lens[b] / pageRows) - 1]; the entries behind them are left as they were.
+ * Calls on one pool change it in place and must be ordered (one stream, or events).  resize and fork
+ * do all of their work or none: with too few free pages, a length beyond the table or a parent
+ * outside the batch the pool stays as it is and the status word (sticky, sharedkv_page_status) says
+ * SHAREDKV_ERANGE.  The reference leaves all of this to the host's block manager. */
+typedef struct PagePoolArgs {
+    uint64_t caches;     /* UINT64 [layers, 2] on the device: base address, bytes between pages
+                            (both multiples of 16)                                        */
+    uint64_t table;      /* INT32 [batch, width]                                         */
+    uint64_t lens;       /* INT32 [batch] rows of each sequence                          */
+    uint64_t refs;       /* INT32 [pages] reference counts                               */
+    uint64_t workspace;  /* >= sharedkv_page_workspace_bytes(batch, width) bytes, 256-aligned, first
+                            256 bytes zeroed once by the owner                           */
+    uint32_t layers, pages, pageRows, batch, width, reserved;
+} PagePoolArgs;
+SHAREDKV_API uint32_t sharedkv_page_args_size(void);
+SHAREDKV_API uint64_t sharedkv_page_workspace_bytes(uint32_t batch, uint32_t width);
+/* Sequence b gets wanted[b] rows (INT32 [batch], device): pages behind the new end lose a reference,
+ * then every sequence that grows takes fresh pages in (sequence, page) order.  A growing sequence
+ * whose last page is partly filled and shared gets a copy of that page in its place. */
+SHAREDKV_API int launch_page_resize(void *stream, const PagePoolArgs *args, const int32_t *wanted);
+/* Sequence b continues sequence parents[b] (INT32 [batch], device; negative: it ends, length 0).
+ * Children share the parent's full pages; the first child keeps its partly filled last page, the
+ * others get copies on fresh pages in sequence order; sequences without a child are released first. */
+SHAREDKV_API int launch_page_fork(void *stream, const PagePoolArgs *args, const int32_t *parents);
+/* Pages pairs[i, 0] -> pairs[i, 1] (INT32 [count, 2], device) in every cache; pairs with an id outside
+ * the pool are skipped.  A page may be copied to several pages; no destination may be named twice or
+ * be a source of the same call.  Uses caches, layers, pages and pageRows only. */
+SHAREDKV_API int launch_page_copy(void *stream, const PagePoolArgs *args, const int32_t *pairs, uint32_t count);
+/* Rows base[b] + kept[b, i] -> base[b] + i (INT32 [batch], [batch, width_kept <= 64], device) in every
+ * cache: the accepted rows of a drafted tree move up behind the committed ones.  Negative entries and
+ * rows without a page are skipped; all rows of a sequence are read before one is written. */
+SHAREDKV_API int launch_page_keep(void *stream, const PagePoolArgs *args, const int32_t *base, const int32_t *kept, uint32_t kept_width);
+/* Host-bridge forms: `op` 0 resize, 1 fork, 2 copy, 3 keep; `a`, `b` the device arrays, `n` the count. */
+SHAREDKV_API int sharedkv_page(uint64_t args, uint32_t op, uint64_t a, uint64_t b, uint32_t n, int32_t device, void *stream);
+/* Synchronises `stream`; SHAREDKV_OK, SHAREDKV_ERANGE (a resize or fork since the workspace was cleared
+ * was refused on the device) or a cudaError_t. */
+SHAREDKV_API int sharedkv_page_status(const void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
