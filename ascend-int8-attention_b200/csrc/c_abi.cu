@@ -159,6 +159,12 @@ int sharedkv_tree_attention(uint64_t args, int32_t device, void *stream)
     return sharedkv::tree_attention(reinterpret_cast<const TreeAttentionArgs *>(args), static_cast<cudaStream_t>(stream));
 }
 
+int sharedkv_tree_status(const void *workspace, void *stream)
+{
+    const int status = sharedkv::page_status(workspace, static_cast<cudaStream_t>(stream));
+    return status == SHAREDKV_ERANGE ? SHAREDKV_ETIMEDOUT : status;
+}
+
 uint32_t sharedkv_page_args_size(void) { return (uint32_t)sizeof(PagePoolArgs); }
 uint64_t sharedkv_page_workspace_bytes(uint32_t batch, uint32_t width) { return sharedkv::page_workspace_bytes(batch, width); }
 int launch_page_resize(void *stream, const PagePoolArgs *args, const int32_t *wanted)

@@ -105,6 +105,20 @@ __device__ __forceinline__ void tma_page_segment(uint32_t dst, const void *tenso
         ::"r"(dst), "l"(tensor_map), "r"(x), "r"(0), "r"(page), "r"(bar)
         : "memory");
 }
+// A box {128 bytes, rows of the map, 1 page} of such a view, from row `row` on.
+__device__ __forceinline__ void tma_page_rows(uint32_t dst, const void *tensor_map, int32_t x, int32_t row, int32_t page, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(tensor_map), "r"(x), "r"(row), "r"(page), "r"(bar)
+        : "memory");
+}
+// Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_descriptor(const void *tensor_map)
 {
     asm volatile("prefetch.tensormap [%0];" ::"l"(tensor_map) : "memory");
@@ -165,6 +179,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr)
         : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4])

@@ -1,13 +1,34 @@
 // Attention of a tree of drafted tokens over the INT8 shared-KV cache, sm_100a.  The contract is in
 // include/sharedkv_c_abi.h.
 //
-// One thread block per (token, eight heads), a warp per head: lane l holds channels 16 l .. 16 l + 15
-// of the scaled query and of the running output.  Keys are taken one by one with an FP32 online
-// softmax (running maximum, sum and output in registers).  Every token fetches its own keys, so the
-// kernel is bound by instruction issue and by L2, far from what the tensor cores allow.
+// What the tokens of a tree have in common is their keys: eight query rows of 8 heads read the same 512-byte
+// key rows as their neighbours in the tree.  So the unit of work is a GROUP of up to 64 query rows of
+// one request (eight OCTETS; an octet is eight consecutive heads of one token), and a 128-key tile is
+// fetched once per group.  A launch is three kernels, four on ratio-4 layers:
+//
+//   tree_encode_kernel   query rows -> two INT8 code planes per cache kind, in the layout of the shared-memory
+//                        operand; group descriptors; rows behind the last live token cleared; its last block
+//                        cuts the launch's tiles into one range per SM
+//   tree_union_kernel    (ratio 4) the top-k lists of a group's tokens -> one ascending list of rows with a
+//                        count per token, through a bitmap, so that rows several tokens name are fetched once
+//   tree_walk_kernel     one persistent block per SM: S = K.Q^T and O = K^T.P on the INT8 tensor cores
+//   tree_merge_kernel    joins the partial results of groups that several SMs worked on
+//
+// Arithmetic of the walk.  f = q * scale, alpha = max|f| / 127, f ~ alpha (q_hi + q_lo / 254); one MMA
+// of 128 keys x (64 hi rows + 64 lo rows) gives both planes, and the integers are joined exactly,
+// S = 254 S_hi + S_lo < 2^31, before the one conversion to FP32.  x = log2(e) s - ref with a reference
+// per row that stays at or above every logit so far; weights 2^x <= 1 become codes c = rint(32639 * 2^x) = 256 c_hi + c_lo
+// (15 bits, c_lo signed), so O = 256 O_hi + O_lo is again one exact integer per tile, summed over tiles in
+// FP32 registers; the denominator is the sum of the same codes.  The reference moves only when some
+// logit exceeds it, and then to two powers of two above that logit (kHeadroom): the exact row maximum, a
+// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  The 2 bits this
+// takes from the codes leave steps of 2^-13 of the largest weight, below a BF16 result's 2^-8.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
 
 #include "../../include/sharedkv_c_abi.h"
 #include "ptx_sm100.cuh"
@@ -16,89 +37,1181 @@
 namespace sharedkv {
 namespace {
 
-using ptx::grid_dependency_launch_dependents;
-using ptx::grid_dependency_wait;
+using namespace ptx;
 
-constexpr uint32_t kTreePage = 32, kTreeDraft = 64, kTreeHeads = 8, kTreeThreads = 256;
+// ------------------------------------------------------------------ geometry
+constexpr uint32_t kTreePage = 32, kTreeDraft = 64;
+constexpr uint32_t kOctet = 8, kGroupOctets = 8, kGroupRows = kOctet * kGroupOctets;
+constexpr uint32_t kCodeRows = 2 * kGroupRows;               // hi plane, then lo plane
+constexpr uint32_t kTile = 128;                              // keys of a tile
+constexpr uint32_t kSeg = kTile * 128;                       // one 128-channel segment of a tile (or of the query codes): 16 KB
+constexpr uint32_t kRing = 8;                                // segments in flight: two tiles
+constexpr uint32_t kWalkThreads = 512;
+constexpr uint32_t kEncodeThreads = 256, kUnionThreads = 1024, kMergeThreads = 256;
+constexpr uint32_t kWarpAccumulate = 4, kWarpIssue = 12, kWarpProduce = 13, kProducers = 3;
+// Registers: launched with 128 per thread; accumulate (two warps of every SM partition) grows to hold
+// 128 running sums a thread, the issuer and the producers shrink.  168 + 168 + 128 + 48 = 4 x 128.
+constexpr uint32_t kRegsAccumulate = 168, kRegsIssue = 48;
+static_assert(2 * kRegsAccumulate + 128 + kRegsIssue <= 4 * 128, "register shares exceed the launch allocation");
+constexpr float kWeightSteps = 32639.f;                      // 127 * 256 + 127: the largest weight code
+constexpr uint32_t kCodeBias = 0x4b000080u;                  // bits of 2^23 + 128
+constexpr float kNoKey = -1e30f;                             // reference of a row that has met no key
+constexpr float kHeadroom = 2.f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows a union bitmap covers at a time (32 KB)
+constexpr uint32_t kTreeWaitMillions = 4000;                 // cycles, ~2 s: a wait that long is a failure
+// Work split, in tiles: what a group costs besides its tiles, and the shortest piece worth a partial result.
+constexpr uint32_t kGroupCost = 2, kMinPiece = 4;
 
-__global__ void __launch_bounds__(kTreeThreads) tree_simple_kernel(const TreeAttentionArgs p)
+// shared memory of the walk (dynamic, 1024-byte aligned, all of the 227 KB)
+constexpr uint32_t kSmKey = 0;
+constexpr uint32_t kSmQuery = kSmKey + kRing * kSeg;         // 64 KB: four segments of 128 code rows
+constexpr uint32_t kSmWeight = kSmQuery + 4 * kSeg;          // two tiles of weight codes, 128 keys x 128 bytes
+constexpr uint32_t kSmAlpha = kSmWeight + 2 * kSeg;          // FP32 [2 kinds][64]
+constexpr uint32_t kSmRef = kSmAlpha + 512;                  // FP32 [64]
+constexpr uint32_t kSmTop = kSmRef + 256;                    // INT32 [64] row maxima, as ordered integers
+constexpr uint32_t kSmFactor = kSmTop + 256;                 // FP32 [2][64] rescale factors of a tile
+constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [64] denominators
+constexpr uint32_t kSmInverse = kSmSum + 256;                // FP32 [64]
+constexpr uint32_t kSmPath = kSmInverse + 256;               // UINT64 [8] paths, UINT64 [8] compressed paths, INT32 [8] path lengths
+constexpr uint32_t kSmFlags = kSmPath + 160;                 // rescale [2], vote [3], page masks [4], tmem base, abort
+constexpr uint32_t kSmBars = kSmFlags + 48;
+constexpr uint32_t kBarKeyFull = 0, kBarKeyEmpty = 8, kBarQueryFull = 16, kBarQueryEmpty = 17, kBarScoreFull = 18, kBarScoreFree = 20,
+                   kBarWeightReady = 22, kBarWeightFree = 24, kBarOutFull = 26, kBarOutFree = 28, kBarSync = 30, kBarDone = 31,
+                   kBarDoneFree = 32, kTreeBars = 33;
+constexpr uint32_t kWalkSmem = kSmBars + 8 * kTreeBars;
+static_assert(kWalkSmem <= 232448, "dynamic shared memory limit of sm_100");
+static_assert(kSmPath % 8 == 0 && kSmBars % 8 == 0, "64-bit words");
+constexpr uint32_t kFlagRescale = 0, kFlagVote = 2, kFlagPages = 5, kFlagTmem = 9, kFlagAbort = 10;
+constexpr uint32_t kTmemAll = 512, kColScore = 0, kColOut = 256;      // two score tiles, two 128-channel blocks of O
+
+struct Group {
+    int32_t request, first_octet, octets, prefix, drafted, ori_tiles, cmp_rows, tiles;
+};
+static_assert(sizeof(Group) == 32, "a descriptor is two 16-byte loads");
+
+// ------------------------------------------------------------------ workspace
+// 256 bytes head (word 0 sticky status, word 1 arrivals of the blocks that prepare the walk), cut points,
+// group descriptors and starts, query codes and alphas, union lists (ratio 4), partial results.
+struct TreeSpace {
+    uint64_t cuts, groups, starts, codes, alphas, rows, counts, partials, bytes;
+    uint32_t octets, slots, kinds;
+};
+__host__ __device__ inline TreeSpace tree_space(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk)
 {
-    __shared__ uint32_t live_batch;
-    grid_dependency_launch_dependents();
-    grid_dependency_wait();
-    const uint32_t lane = threadIdx.x & 31u, head = blockIdx.y * kTreeHeads + (threadIdx.x >> 5), t = blockIdx.x;
-    const int32_t *cu = reinterpret_cast<const int32_t *>(p.cuQ), *seq = reinterpret_cast<const int32_t *>(p.seqLens);
-    if (threadIdx.x == 0) live_batch = 0;
+    TreeSpace s;
+    s.octets = tokens * (heads / kOctet);
+    s.slots = s.octets / kGroupOctets + batch + 1u;           // see slot_of
+    s.kinds = ratio == 1u ? 1u : 2u;
+    auto up = [](uint64_t v) { return (v + 255ull) & ~255ull; };
+    s.cuts = 256;
+    s.groups = up(s.cuts + 8ull * (split::kMaxCtas + 1u));
+    s.starts = up(s.groups + 32ull * s.slots);
+    s.codes = up(s.starts + 4ull * (s.slots + 1u));
+    s.alphas = up(s.codes + 8192ull * s.kinds * s.octets);
+    s.rows = up(s.alphas + 32ull * s.kinds * s.octets);
+    const uint64_t entries = ratio == 4u ? (uint64_t)s.octets * topk : 0ull;
+    s.counts = up(s.rows + 4ull * entries);
+    s.partials = up(s.counts + 16ull * entries);
+    s.bytes = s.partials + 2ull * split::kMaxCtas * (kGroupRows * (kDim + 2ull)) * 4ull;
+    return s;
+}
+constexpr uint32_t kPartial = kGroupRows * (kDim + 2);        // FP32: output sums [64][512], denominators [64], references [64]
+
+struct Tree {
+    TreeAttentionArgs a;
+    TreeSpace s;
+    uint32_t grid;                 // blocks of the walk
+    __device__ __forceinline__ char *at(uint64_t offset) const { return reinterpret_cast<char *>(a.workspace) + offset; }
+    __device__ __forceinline__ const int32_t *cu() const { return reinterpret_cast<const int32_t *>(a.cuQ); }
+    __device__ __forceinline__ const int32_t *seq() const { return reinterpret_cast<const int32_t *>(a.seqLens); }
+    __device__ __forceinline__ Group *groups() const { return reinterpret_cast<Group *>(at(s.groups)); }
+    __device__ __forceinline__ uint32_t *head() const { return reinterpret_cast<uint32_t *>(a.workspace); }
+};
+
+// Descriptor slot of the j-th group of request b.  floor(x + y) + 1 >= floor(x) + ceil(y), so requests
+// do not run into each other and the slots are in request order; the ones between stay empty.
+__device__ __forceinline__ uint32_t slot_of(uint32_t octets_before, uint32_t request, uint32_t j) { return octets_before / kGroupOctets + request + j; }
+
+// Live requests and tokens (trailing requests without rows or with a negative cumulative count are padding).
+__device__ uint32_t live_requests(const Tree &p, uint32_t *shared)
+{
+    if (threadIdx.x == 0) *shared = 0;
     __syncthreads();
     uint32_t live = 0;
-    for (uint32_t b = threadIdx.x; b < p.batch; b += kTreeThreads) if (split::request_is_live(seq[b], cu[b + 1])) live = b + 1;
-    if (live) atomicMax(&live_batch, live);
+    for (uint32_t b = threadIdx.x; b < p.a.batch; b += blockDim.x) if (split::request_is_live(p.seq()[b], p.cu()[b + 1])) live = b + 1;
+    live = __reduce_max_sync(0xffffffffu, live);
+    if (live && (threadIdx.x & 31u) == 0) atomicMax(shared, live);
     __syncthreads();
-    const uint32_t live_tokens = split::live_token_count(live_batch ? cu[live_batch] : 0, p.tokens);
-    __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.out) + ((uint64_t)t * p.heads + head) * kDim + lane * 16u;
-    float *lse = p.lse ? reinterpret_cast<float *>(p.lse) + (uint64_t)t * p.heads + head : nullptr;
-    if (t >= live_tokens || (int32_t)t < cu[0]) {
-        reinterpret_cast<uint4 *>(out)[0] = reinterpret_cast<uint4 *>(out)[1] = make_uint4(0, 0, 0, 0);
-        if (lse && lane == 0) *lse = 0.f;
-        return;
-    }
-    uint32_t b = 0, hi = live_batch - 1;
-    while (b < hi) {
-        const uint32_t mid = (b + hi) >> 1;
-        if (cu[mid + 1] <= (int32_t)t) b = mid + 1; else hi = mid;
-    }
-    const int32_t n = cu[b + 1] - cu[b];
-    const int64_t prefix = (int64_t)seq[b] - n;
-    uint64_t path = reinterpret_cast<const uint64_t *>(p.paths)[t];
-    if (n < (int32_t)kTreeDraft) path &= (1ull << n) - 1ull;
-    const int64_t c = __popcll(path);
+    return *shared;
+}
 
-    float q[16], sc[2][16], acc[16], m = -INFINITY, l = 0.f;
-    const __nv_bfloat16 *qs = reinterpret_cast<const __nv_bfloat16 *>(p.q) + ((uint64_t)t * p.heads + head) * kDim + lane * 16u;
-    for (int i = 0; i < 16; ++i) {
-        q[i] = __bfloat162float(qs[i]) * p.softmaxScale;
-        sc[0][i] = reinterpret_cast<const float *>(p.oriScale)[lane * 16u + i];
-        sc[1][i] = reinterpret_cast<const float *>(p.cmpScale)[lane * 16u + i];
-        acc[i] = 0.f;
-    }
-    auto attend = [&](int kind, int64_t row) {
-        const uint32_t width = kind ? p.cmpTableWidth : p.oriTableWidth, pages = kind ? p.cmpPages : p.oriPages;
-        if (row < 0 || row / kTreePage >= width) return;
-        const int32_t page = reinterpret_cast<const int32_t *>(kind ? p.cmpTable : p.oriTable)[(uint64_t)b * width + row / kTreePage];
-        if ((uint32_t)page >= pages) return;
-        const uint64_t src = (kind ? p.cmp : p.ori) + (uint64_t)page * (kind ? p.cmpStride : p.oriStride) + (uint64_t)(row % kTreePage) * kDim;
-        const uint4 raw = *reinterpret_cast<const uint4 *>(src + lane * 16u);
-        const int8_t *codes = reinterpret_cast<const int8_t *>(&raw);
-        float v[16], s = 0.f;
-        for (int i = 0; i < 16; ++i) { v[i] = (float)codes[i] * sc[kind][i]; s = fmaf(q[i], v[i], s); }
-        for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const float top = fmaxf(m, s), r = m == -INFINITY ? 0.f : expf(m - top), w = expf(s - top);
-        l = fmaf(l, r, w);
-        for (int i = 0; i < 16; ++i) acc[i] = fmaf(acc[i], r, w * v[i]);
-        m = top;
+// Rows of the union of a request's windows start at a page: the committed rows a path without a bit sees.
+__device__ __forceinline__ int32_t window_page(int32_t prefix, uint32_t window)
+{
+    return prefix > (int32_t)window ? (prefix - (int32_t)window) / (int32_t)kTreePage : 0;
+}
+
+// ------------------------------------------------------------------ work split
+// Runs in the last block of the kernel in front of the walk.  The tiles of all groups, each group with
+// kGroupCost units in front, are cut into p.grid ranges of equal cost; a cut that would leave a piece of fewer than
+// kMinPiece tiles moves to the group's edge.  Cut i is (slot, tile): block i walks from cut i to cut i + 1.
+__device__ void cut_tiles(const Tree &p)
+{
+    __shared__ uint32_t sums[33];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x / 32u;
+    uint32_t *starts = reinterpret_cast<uint32_t *>(p.at(p.s.starts));
+    const uint32_t per = (p.s.slots + blockDim.x - 1u) / blockDim.x;
+    const uint32_t begin = min(threadIdx.x * per, p.s.slots), end = min(begin + per, p.s.slots);
+    auto cost = [&](uint32_t slot) {
+        const uint32_t tiles = (uint32_t)__ldcg(&p.groups()[slot].tiles);
+        return tiles ? tiles + kGroupCost : 0u;
     };
-    for (int64_t r = max((int64_t)0, prefix - (int64_t)p.window + c); r < prefix; ++r) attend(0, r);
-    for (uint64_t left = path; left; left &= left - 1ull) attend(0, prefix + __ffsll((long long)left) - 1);
-    const int64_t whole = prefix > 0 ? prefix / p.ratio : 0;
-    if (p.ratio == 128u) {
-        for (int64_t r = 0; r < whole; ++r) attend(1, r);
-        if (p.cmpPaths)
-            for (uint64_t left = reinterpret_cast<const uint64_t *>(p.cmpPaths)[t]; left; left &= left - 1ull) attend(1, whole + __ffsll((long long)left) - 1);
-    } else if (p.ratio == 4u) {
-        for (uint32_t i = 0; i < p.topk; ++i) {
-            const int32_t r = reinterpret_cast<const int32_t *>(p.indices)[(uint64_t)t * p.topk + i];
-            if (r >= 0 && r < whole + kTreeDraft) attend(1, r);
+    uint32_t sum = 0;
+    for (uint32_t i = begin; i < end; ++i) sum += cost(i);
+    uint32_t incl = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t n = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= (uint32_t)d) incl += n;
+    }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t s = lane < warps ? sums[lane] : 0u;
+        uint32_t si = s;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t n = __shfl_up_sync(0xffffffffu, si, d);
+            if (lane >= (uint32_t)d) si += n;
+        }
+        sums[lane] = si - s;
+        if (lane == 31) sums[32] = si;
+    }
+    __syncthreads();
+    uint32_t before = sums[warp] + incl - sum;
+    for (uint32_t i = begin; i < end; ++i) { starts[i] = before; before += cost(i); }
+    const uint32_t total = sums[32];
+    if (threadIdx.x == 0) starts[p.s.slots] = total;
+    __syncthreads();
+    const uint32_t quota = total ? (total + p.grid - 1u) / p.grid : 1u;
+    uint2 *cuts = reinterpret_cast<uint2 *>(p.at(p.s.cuts));
+    for (uint32_t i = threadIdx.x; i <= p.grid; i += blockDim.x) {
+        const uint32_t position = i * quota;
+        if (i == p.grid || position >= total) { cuts[i] = make_uint2(p.s.slots, 0); continue; }
+        uint32_t lo = 0, hi = p.s.slots - 1u;                 // last slot that starts at or before the position
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi + 1u) >> 1;
+            if (starts[mid] <= position) lo = mid; else hi = mid - 1u;
+        }
+        const uint32_t inside = position - starts[lo], tiles = starts[lo + 1u] - starts[lo] - kGroupCost;
+        const uint32_t tile = inside > kGroupCost ? inside - kGroupCost : 0u;
+        cuts[i] = tile < kMinPiece ? make_uint2(lo, 0) : tiles - tile < kMinPiece ? make_uint2(lo + 1u, 0) : make_uint2(lo, tile);
+    }
+}
+
+// One arrival per block; true in the block that arrives last, which sees what the others wrote.
+__device__ bool last_block(const Tree &p, uint32_t blocks)
+{
+    __shared__ uint32_t mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        mine = atomic_add_acq_rel(p.head() + 1, 1u);
+        if (mine + 1u == blocks) p.head()[1] = 0;             // as the next launch needs it
+    }
+    __syncthreads();
+    return mine + 1u == blocks;
+}
+
+// ------------------------------------------------------------------ encode
+// One block per octet, a warp per head: lane l owns channels 16 l .. 16 l + 15, one 16-byte chunk of a code
+// row.  Codes go out as the walk's B operand wants them: [kind][segment][plane][octet] blocks of 8 rows x
+// 128 bytes, swizzled, so that a group's rows of a plane are one contiguous copy.
+__device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_t octet, uint32_t row, const float (&q)[16])
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    const float *scale = reinterpret_cast<const float *>(kind ? p.a.cmpScale : p.a.oriScale) + lane * 16u;
+    float f[16];
+    uint32_t top = 0;                                         // largest |f| as an integer: a NaN or an infinity wins
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        f[i] = q[i] * __ldg(scale + i);
+        top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    const bool finite = top < 0x7f800000u;
+    const float alpha = fmaxf(__uint_as_float(top) * (float)(1.0 / 127), 1e-30f), rcp = __frcp_rn(alpha);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        // adding 1.5 * 2^23 leaves the nearest integer in the low bits of the sum
+        uint32_t ch[4], cl[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float n = f[4 * w + e] * rcp, shifted = __fadd_rn(n, 12582912.f), rest = __fsub_rn(n, __fsub_rn(shifted, 12582912.f));
+            ch[e] = __float_as_uint(shifted);
+            cl[e] = __float_as_uint(__fadd_rn(__fmul_rn(rest, 254.f), 12582912.f));
+        }
+        hi[w] = __byte_perm(__byte_perm(ch[0], ch[1], 0x0040), __byte_perm(ch[2], ch[3], 0x0040), 0x5410);
+        lo[w] = __byte_perm(__byte_perm(cl[0], cl[1], 0x0040), __byte_perm(cl[2], cl[3], 0x0040), 0x5410);
+    }
+    const uint64_t plane = 1024ull * p.s.octets, segment = kind * 4u + (lane >> 3);
+    char *dst = p.at(p.s.codes) + segment * 2ull * plane + 1024ull * octet + row * 128u + (((lane & 7u) ^ row) << 4);
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4 *>(dst + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (lane == 0)
+        reinterpret_cast<float *>(p.at(p.s.alphas))[(uint64_t)(kind * p.s.octets + octet) * kOctet + row] =
+            finite ? alpha * p.a.softmaxScale * (kLog2e / 254.f) : __uint_as_float(0x7fc00000u);
+}
+
+__global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __grid_constant__ Tree p)
+{
+    __shared__ uint32_t shared_live;
+    grid_dependency_launch_dependents();
+    grid_dependency_wait();
+    const uint32_t lane = threadIdx.x & 31u, row = threadIdx.x >> 5, octet = blockIdx.x, per_token = p.a.heads / kOctet;
+    const int32_t *cu = p.cu();
+    const uint32_t token = octet / per_token;
+    const uint4 *src = reinterpret_cast<const uint4 *>(p.a.q + ((uint64_t)octet * kOctet + row) * (kDim * 2u)) + lane * 2u;
+    const uint4 raw[2] = {src[0], src[1]};                    // in flight while the block finds out whose row it is
+    const uint32_t live = live_requests(p, &shared_live);
+    const uint32_t live_tokens = split::live_token_count(live ? cu[live] : 0, p.a.tokens);
+    // slots of no group: the empty ones between requests, and those behind the last
+    for (uint32_t i = blockIdx.x * kEncodeThreads + threadIdx.x; i < p.s.slots; i += gridDim.x * kEncodeThreads) {
+        uint32_t lo = 0, hi = live ? live - 1u : 0u;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi + 1u) >> 1;
+            if (slot_of((uint32_t)max(cu[mid], 0) * per_token, mid, 0) <= i) lo = mid; else hi = mid - 1u;
+        }
+        Group g = {};
+        if (live) {
+            const int32_t first = max(cu[lo], 0), n = min(cu[lo + 1], (int32_t)live_tokens) - first;
+            const uint32_t base = slot_of((uint32_t)first * per_token, lo, 0), octets = n > 0 ? (uint32_t)n * per_token : 0u;
+            if (i >= base && (i - base) * kGroupOctets < octets) {
+                const uint32_t j = i - base;
+                g.request = (int32_t)lo;
+                g.first_octet = (int32_t)((uint32_t)first * per_token + j * kGroupOctets);
+                g.octets = (int32_t)min(kGroupOctets, octets - j * kGroupOctets);
+                g.prefix = p.seq()[lo] - (cu[lo + 1] - cu[lo]);
+                g.drafted = min(n, (int32_t)kTreeDraft);
+                const int64_t last = (int64_t)g.prefix + g.drafted, start = (int64_t)window_page(g.prefix, p.a.window) * kTreePage;
+                // one tile at least, so that the rows of a group without a key are written
+                g.ori_tiles = last > start ? (int32_t)((last - start + kTile - 1) / kTile) : 1;
+                const int64_t table_rows = (int64_t)p.a.cmpTableWidth * kTreePage;
+                int64_t rows = 0;
+                if (p.a.ratio == 128u) rows = (int64_t)(max(g.prefix, 0) / 128) + (p.a.cmpPaths ? (int32_t)kTreeDraft : 0);
+                g.cmp_rows = (int32_t)(rows < table_rows ? rows : table_rows);
+                g.tiles = g.ori_tiles + (g.cmp_rows + (int32_t)kTile - 1) / (int32_t)kTile;
+            }
+        }
+        p.groups()[i] = g;
+    }
+    if (token >= live_tokens || (int32_t)token < cu[0]) {
+        const uint64_t at = ((uint64_t)octet * kOctet + row) * kDim;
+        uint4 *out = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.a.out) + at) + lane * 2u;
+        out[0] = out[1] = make_uint4(0, 0, 0, 0);
+        if (p.a.lse && lane == 0) reinterpret_cast<float *>(p.a.lse)[(uint64_t)octet * kOctet + row] = 0.f;
+    } else {
+        float q[16];
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { q[2 * i] = __uint_as_float(words[i] << 16); q[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u); }
+#pragma unroll 1
+        for (uint32_t kind = 0; kind < p.s.kinds; ++kind) encode_row(p, kind, octet, row, q);
+    }
+    if (p.a.ratio != 4u && last_block(p, gridDim.x)) cut_tiles(p);
+}
+
+// ------------------------------------------------------------------ union of top-k lists
+// One block per group.  Rows are ranked by the bits before theirs in a bitmap, so the list ascends whatever
+// order the atomics ran in.  An entry carries its location (page * 32 + row in page, -1 when the page
+// is missing) and, per octet, how often the octet's token names it.
+__global__ void __launch_bounds__(kUnionThreads, 1) tree_union_kernel(const __grid_constant__ Tree p)
+{
+    extern __shared__ uint32_t smem[];
+    uint32_t *bitmap = smem, *base = bitmap + kUnionRows / 32u, *counts = base + kUnionRows / 32u;      // counts: UINT16 [entries][8]
+    __shared__ uint32_t sums[33];
+    grid_dependency_launch_dependents();
+    grid_dependency_wait();
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, per_token = p.a.heads / kOctet;
+    const Group g = p.groups()[blockIdx.x];
+    if (g.octets) {
+        const uint32_t first_token = (uint32_t)g.first_octet / per_token;
+        const uint32_t tokens = ((uint32_t)(g.first_octet + g.octets) - 1u) / per_token - first_token + 1u;
+        const uint32_t total = tokens * p.a.topk;             // at most 8 x 1024: eight entries a thread
+        const int64_t table_rows = (int64_t)p.a.cmpTableWidth * kTreePage, named = (int64_t)(max(g.prefix, 0) / 4) + kTreeDraft;
+        const uint32_t limit = (uint32_t)(named < table_rows ? named : table_rows);
+        const int32_t *picks = reinterpret_cast<const int32_t *>(p.a.indices) + (uint64_t)first_token * p.a.topk;
+        const int32_t *table = reinterpret_cast<const int32_t *>(p.a.cmpTable) + (uint64_t)g.request * p.a.cmpTableWidth;
+        const uint64_t at = (uint64_t)g.first_octet * p.a.topk;
+        int32_t *rows_out = reinterpret_cast<int32_t *>(p.at(p.s.rows)) + at;
+        uint4 *counts_out = reinterpret_cast<uint4 *>(p.at(p.s.counts)) + at;
+        uint32_t pick[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            const uint32_t i = threadIdx.x + k * kUnionThreads;
+            const uint32_t v = i < total ? (uint32_t)picks[i] : 0xffffffffu;
+            pick[k] = v < limit ? v : 0xffffffffu;
+        }
+        uint32_t listed = 0;
+        for (uint32_t low = 0; low < limit; low += kUnionRows) {
+            const uint32_t words = (min(limit - low, kUnionRows) + 31u) / 32u;
+            for (uint32_t i = threadIdx.x; i < words; i += kUnionThreads) bitmap[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t r = pick[k] - low;
+                if (pick[k] != 0xffffffffu && pick[k] >= low && r < kUnionRows) atomicOr(bitmap + r / 32u, 1u << (r & 31u));
+            }
+            __syncthreads();
+            const uint32_t per = (words + kUnionThreads - 1u) / kUnionThreads;
+            const uint32_t begin = min(threadIdx.x * per, words), end = min(begin + per, words);
+            uint32_t sum = 0;
+            for (uint32_t i = begin; i < end; ++i) sum += __popc(bitmap[i]);
+            uint32_t incl = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t n = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= (uint32_t)d) incl += n;
+            }
+            if (lane == 31) sums[warp] = incl;
+            __syncthreads();
+            if (warp == 0) {
+                const uint32_t s = sums[lane];
+                uint32_t si = s;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t n = __shfl_up_sync(0xffffffffu, si, d);
+                    if (lane >= (uint32_t)d) si += n;
+                }
+                sums[lane] = si - s;
+                if (lane == 31) sums[32] = si;
+            }
+            __syncthreads();
+            uint32_t before = sums[warp] + incl - sum;
+            const uint32_t found = sums[32];
+            for (uint32_t i = begin; i < end; ++i) {
+                base[i] = before;
+                uint32_t bits = bitmap[i];
+                while (bits) {
+                    const uint32_t r = low + i * 32u + (uint32_t)__ffs((int)bits) - 1u;
+                    const int32_t page = table[r / kTreePage];
+                    rows_out[listed + before] = (uint32_t)page < p.a.cmpPages ? (int32_t)((uint32_t)page * kTreePage + (r % kTreePage)) : -1;
+                    ++before;
+                    bits &= bits - 1u;
+                }
+            }
+            for (uint32_t i = threadIdx.x; i < found * 4u; i += kUnionThreads) counts[i] = 0;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                const uint32_t r = pick[k] - low;
+                if (pick[k] == 0xffffffffu || pick[k] < low || r >= kUnionRows) continue;
+                const uint32_t rank = base[r / 32u] + __popc(bitmap[r / 32u] & ((1u << (r & 31u)) - 1u));
+                const uint32_t token = first_token + (threadIdx.x + k * kUnionThreads) / p.a.topk;
+                const int32_t o0 = max((int32_t)(token * per_token) - g.first_octet, 0);
+                const int32_t o1 = min((int32_t)((token + 1u) * per_token) - g.first_octet, g.octets);
+                for (int32_t o = o0; o < o1; ++o) atomicAdd(counts + rank * 4u + (uint32_t)o / 2u, (o & 1) ? 0x10000u : 1u);
+            }
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < found; i += kUnionThreads) counts_out[listed + i] = reinterpret_cast<const uint4 *>(counts)[i];
+            listed += found;
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) {
+            p.groups()[blockIdx.x].cmp_rows = (int32_t)listed;
+            p.groups()[blockIdx.x].tiles = g.ori_tiles + (int32_t)((listed + kTile - 1u) / kTile);
         }
     }
-    const float sink = reinterpret_cast<const float *>(p.sinks)[head], top = fmaxf(m, sink);
-    const float r = m == -INFINITY ? 0.f : expf(m - top), total = l * r + (sink == -INFINITY ? 0.f : expf(sink - top));
-    for (int i = 0; i < 16; ++i) out[i] = __float2bfloat16_rn(total > 0.f || total != total ? acc[i] * r / total : 0.f);
-    if (lse && lane == 0) *lse = total > 0.f || total != total ? top + logf(total) : -INFINITY;
+    if (last_block(p, gridDim.x)) cut_tiles(p);
+}
+
+// ------------------------------------------------------------------ walk: common to the roles
+struct WalkShared {
+    uint32_t base;
+    char *ptr;
+    __device__ __forceinline__ uint32_t bar(uint32_t i) const { return base + kSmBars + 8u * i; }
+    __device__ __forceinline__ volatile uint32_t *flags() const { return reinterpret_cast<volatile uint32_t *>(ptr + kSmFlags); }
+    __device__ __forceinline__ float *floats(uint32_t offset) const { return reinterpret_cast<float *>(ptr + offset); }
+};
+
+// A bounded wait: false once a wait of the block has run out.  One copy of the polling loop per ROLE, because
+// warps with different register allocations cannot share a function.
+template <int ROLE>
+__device__ __noinline__ bool walk_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *flags)
+{
+    const long long start = clock64();
+#pragma unroll 1
+    for (uint32_t spin = 1;; ++spin) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((spin & 63u) == 0) {
+            if (flags[kFlagAbort]) return false;
+            if (clock64() - start > (long long)kTreeWaitMillions * 1000000ll) { flags[kFlagAbort] = 1; return false; }
+        }
+    }
+}
+template <int ROLE>
+__device__ __forceinline__ bool walk_wait(const WalkShared &sm, uint32_t bar_index, uint32_t parity)
+{
+    const uint32_t bar = sm.bar(bar_index);
+    if (mbar_try_wait(bar, parity)) return true;
+    return walk_wait_slow<ROLE>(bar, parity, sm.flags());
+}
+
+// The block's items in order: groups, the first and last possibly in part.  The next descriptor is
+// read while the current item is worked on.
+struct Items {
+    uint32_t slot, last_slot, last_tile, begin, end;
+    Group g, next;
+    __device__ __forceinline__ Group load(const Tree &p, uint32_t at) const
+    {
+        Group v = {};
+        if (at < p.s.slots) {
+            const int4 *src = reinterpret_cast<const int4 *>(p.groups() + at);
+            const int4 a = __ldcg(src), b = __ldcg(src + 1);
+            v.request = a.x; v.first_octet = a.y; v.octets = a.z; v.prefix = a.w;
+            v.drafted = b.x; v.ori_tiles = b.y; v.cmp_rows = b.z; v.tiles = b.w;
+        }
+        return v;
+    }
+    __device__ __forceinline__ bool open(const Tree &p, uint32_t from)
+    {
+        for (;; from = 0) {
+            end = slot == last_slot ? last_tile : (uint32_t)g.tiles;
+            begin = from;
+            if (slot >= p.s.slots || slot > last_slot) return false;
+            if (begin < end) return true;
+            g = next;
+            ++slot;
+            next = load(p, slot + 1u);
+        }
+    }
+    __device__ __forceinline__ bool first(const Tree &p)
+    {
+        const uint2 *cuts = reinterpret_cast<const uint2 *>(p.at(p.s.cuts)) + blockIdx.x;
+        const uint2 a = __ldcg(cuts), b = __ldcg(cuts + 1);
+        slot = a.x; last_slot = b.x; last_tile = b.y;
+        g = load(p, slot);
+        next = load(p, slot + 1u);
+        return open(p, a.y);
+    }
+    __device__ __forceinline__ bool advance(const Tree &p)
+    {
+        g = next;
+        ++slot;
+        next = load(p, slot + 1u);
+        return open(p, 0u);
+    }
+    __device__ __forceinline__ bool whole() const { return begin == 0 && end == (uint32_t)g.tiles; }
+    // Partial results: a block has at most one piece that another block continues and one that continues
+    // another's, hence two places per block.
+    __device__ __forceinline__ uint32_t partial() const { return 2u * blockIdx.x + (begin == 0 ? 1u : 0u); }
+};
+
+// ------------------------------------------------------------------ walk: producers
+// Three warps take the segments of the tiles in turn: 128 channels of 128 keys, 16 KB.  Pages come as
+// whole boxes of 32 rows x 128 bytes; the listed rows of a ratio-4 layer by gathers of four rows, or
+// row by row when the page stride is no multiple of a row.
+template <bool LISTED>
+__device__ void produce(const Tree &p, const WalkShared &sm, uint32_t mine, const CUtensorMap *ori_map, const CUtensorMap *cmp_map,
+                        const CUtensorMap *row_map, bool gather)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    Items it;
+    uint32_t tile = 0, turn = 0;                              // tiles of the block so far; segment number modulo kProducers
+    for (bool more = it.first(p); more; more = it.advance(p)) {
+        for (uint32_t j = it.begin; j < it.end; ++j, ++tile) {
+            const bool ori = j < (uint32_t)it.g.ori_tiles;
+            if (LISTED && !ori) {
+                // lane l fetches rows 4 l .. 4 l + 3 of the tile
+                const uint32_t row = (j - (uint32_t)it.g.ori_tiles) * kTile + 4u * lane;
+                const int32_t *list = reinterpret_cast<const int32_t *>(p.at(p.s.rows)) + (uint64_t)it.g.first_octet * p.a.topk;
+                int32_t at[4];
+                uint32_t there = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    at[i] = row + i < (uint32_t)it.g.cmp_rows ? __ldcg(list + row + i) : -1;
+                    there += at[i] >= 0;
+                }
+                const uint32_t per_page = (uint32_t)(p.a.cmpStride / kDim);
+                const uint32_t bytes = gather ? 512u * __popc(__ballot_sync(0xffffffffu, there != 0))
+                                              : 128u * __reduce_add_sync(0xffffffffu, there);
+#pragma unroll 1
+                for (uint32_t seg = 0; seg < 4; ++seg) {
+                    const bool take = turn == mine;
+                    turn = turn + 1u == kProducers ? 0u : turn + 1u;
+                    if (!take) continue;
+                    const uint32_t slot = (4u * tile + seg) % kRing;
+                    if (!walk_wait<2>(sm, kBarKeyEmpty + slot, ((tile >> 1) & 1u) ^ 1u)) return;
+                    if (lane == 0) mbar_arrive_expect_tx(sm.bar(kBarKeyFull + slot), bytes);
+                    __syncwarp();
+                    const uint32_t dst = sm.base + kSmKey + slot * kSeg + lane * 512u;
+                    if (gather) {
+                        int32_t r[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)           // a missing row reads as zeros from beyond the map
+                            r[i] = at[i] < 0 ? 0x7ffffff0 : (int32_t)((uint32_t)at[i] / kTreePage * per_page + (uint32_t)at[i] % kTreePage);
+                        if (there) tma_gather4(dst, row_map, (int32_t)(seg * 128u), r[0], r[1], r[2], r[3], sm.bar(kBarKeyFull + slot));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (at[i] >= 0)
+                                tma_page_rows(dst + i * 128u, row_map, (int32_t)(seg * 128u), at[i] % (int32_t)kTreePage, at[i] / (int32_t)kTreePage,
+                                              sm.bar(kBarKeyFull + slot));
+                    }
+                }
+            } else {
+                // lane l < 4 fetches the tile's l-th page
+                const int32_t *table = reinterpret_cast<const int32_t *>(ori ? p.a.oriTable : p.a.cmpTable);
+                const uint32_t width = ori ? p.a.oriTableWidth : p.a.cmpTableWidth;
+                const uint32_t index = (ori ? (uint32_t)window_page(it.g.prefix, p.a.window) + j * 4u : (j - (uint32_t)it.g.ori_tiles) * 4u) + lane;
+                int32_t page = -1;
+                if (lane < 4 && index < width) page = table[(uint64_t)it.g.request * width + index];
+                const bool there = (uint32_t)page < (ori ? p.a.oriPages : p.a.cmpPages);
+                const uint32_t mask = __ballot_sync(0xffffffffu, there) & 15u;
+#pragma unroll 1
+                for (uint32_t seg = 0; seg < 4; ++seg) {
+                    const bool take = turn == mine;
+                    turn = turn + 1u == kProducers ? 0u : turn + 1u;
+                    if (!take) continue;
+                    const uint32_t slot = (4u * tile + seg) % kRing;
+                    if (!walk_wait<2>(sm, kBarKeyEmpty + slot, ((tile >> 1) & 1u) ^ 1u)) return;
+                    if (lane == 0) {
+                        if (seg == 0) sm.flags()[kFlagPages + (tile & 3u)] = mask;
+                        mbar_arrive_expect_tx(sm.bar(kBarKeyFull + slot), 4096u * __popc(mask));
+                    }
+                    __syncwarp();
+                    if (lane < 4 && there)
+                        tma_page_rows(sm.base + kSmKey + slot * kSeg + lane * 4096u, ori ? ori_map : cmp_map, (int32_t)(seg * 128u), 0, page,
+                                      sm.bar(kBarKeyFull + slot));
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ walk: issue
+// One warp issues both products (its elected lane; the warp stays converged).  The scores of tile t + 1
+// go out before the output product of tile t, which waits for the weights, so the tensor core works while the
+// softmax does.  The query codes of an item's kind are one resident set of 64 KB; they are replaced
+// once the last score product that reads them has completed.
+__device__ void issue(const Tree &p, const WalkShared &sm, uint32_t tmem)
+{
+    constexpr uint32_t kScore = idesc_i8(128, kCodeRows, 0, 0), kOut = idesc_i8(128, kCodeRows, 1, 1);
+    const bool leader = elect_one();
+    auto output_product = [&](uint32_t t) {
+        const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
+        if (!walk_wait<3>(sm, kBarWeightReady + buf, ph)) return false;
+        const uint64_t b0 = smem_desc(sm.base + kSmWeight + buf * kSeg, kSeg, 1024u, kSwizzle128);
+#pragma unroll 1
+        for (uint32_t block = 0; block < 4; ++block) {
+            const uint32_t half = block & 1u, use = 2u * t + (block >> 1), slot = (4u * t + block) % kRing;
+            if (!walk_wait<3>(sm, kBarOutFree + half, (use & 1u) ^ 1u)) return false;
+            tc_fence_after();
+            const uint64_t a0 = smem_desc(sm.base + kSmKey + slot * kSeg, kSeg, 1024u, kSwizzle128);
+            if (leader) {
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k)
+                    mma_i8(tmem + kColOut + half * kCodeRows, a0 + ((k * 4096u) >> 4), b0 + ((k * 4096u) >> 4), kOut, k);
+                mma_commit(sm.bar(kBarOutFull + half));
+                mma_commit(sm.bar(kBarKeyEmpty + slot));      // the segment's last reader
+                if (block == 3) mma_commit(sm.bar(kBarWeightFree + buf));
+            }
+            __syncwarp();
+        }
+        return true;
+    };
+    Items it;
+    uint32_t t = 0, sets = 0;
+    for (bool more = it.first(p); more; more = it.advance(p)) {
+        for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
+            const uint32_t ori_tiles = (uint32_t)it.g.ori_tiles, kind = j < ori_tiles ? 0u : 1u;
+            if (j == it.begin || j == ori_tiles) {
+                if (sets && !walk_wait<3>(sm, kBarQueryEmpty, (sets - 1u) & 1u)) return;
+                const uint32_t bytes = 1024u * (uint32_t)it.g.octets;
+                if (leader) {
+                    mbar_arrive_expect_tx(sm.bar(kBarQueryFull), 8u * bytes);
+                    const uint64_t plane = 1024ull * p.s.octets;
+                    const char *src = p.at(p.s.codes) + kind * 8ull * plane + 1024ull * (uint32_t)it.g.first_octet;
+#pragma unroll 1
+                    for (uint32_t i = 0; i < 8; ++i)
+                        bulk_load(sm.base + kSmQuery + (i >> 1) * kSeg + (i & 1u) * (kSeg / 2u), src + i * plane, bytes, sm.bar(kBarQueryFull));
+                }
+                __syncwarp();
+                if (!walk_wait<3>(sm, kBarQueryFull, sets & 1u)) return;
+                ++sets;
+            }
+            const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
+            if (!walk_wait<3>(sm, kBarScoreFree + buf, ph ^ 1u)) return;
+            tc_fence_after();
+#pragma unroll 1
+            for (uint32_t seg = 0; seg < 4; ++seg) {
+                const uint32_t slot = (4u * t + seg) % kRing;
+                if (!walk_wait<3>(sm, kBarKeyFull + slot, ph)) return;
+                const uint64_t a0 = smem_desc(sm.base + kSmKey + slot * kSeg, 16u, 1024u, kSwizzle128);
+                const uint64_t b0 = smem_desc(sm.base + kSmQuery + seg * kSeg, 16u, 1024u, kSwizzle128);
+                if (leader) {
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k)
+                        mma_i8(tmem + kColScore + buf * kCodeRows, a0 + ((k * 32u) >> 4), b0 + ((k * 32u) >> 4), kScore, seg | k);
+                }
+                __syncwarp();
+            }
+            if (leader) {
+                mma_commit(sm.bar(kBarScoreFull + buf));
+                if (j + 1u == it.end || j + 1u == ori_tiles) mma_commit(sm.bar(kBarQueryEmpty));
+            }
+            __syncwarp();
+            if (t && !output_product(t - 1u)) return;
+        }
+    }
+    if (t) output_product(t - 1u);
+}
+
+// ------------------------------------------------------------------ walk: softmax (warps 0-3)
+// Thread = key of the tile; it holds the key's 64 logits.  Sums over keys (the denominators) and, when a
+// logit exceeds its row's reference, maxima over keys are warp reductions of integers, whose
+// result does not depend on their order.
+__device__ __forceinline__ bool softmax_sync(const WalkShared &sm, uint32_t &phase)
+{
+    mbar_arrive(sm.bar(kBarSync));
+    const bool ok = walk_wait<0>(sm, kBarSync, phase);
+    phase ^= 1u;
+    return ok;
+}
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Integers in the order of the floats they come from (and back).
+__device__ __forceinline__ int32_t ordered(int32_t bits) { return bits ^ ((bits >> 31) & 0x7fffffff); }
+
+template <bool LISTED>
+__device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
+{
+    const uint32_t key = threadIdx.x, lane = key & 31u, warp = key >> 5;
+    const uint32_t tmem_lane = tmem + ((warp * 32u) << 16);
+    volatile uint32_t *flags = sm.flags();
+    float *alpha = sm.floats(kSmAlpha), *ref = sm.floats(kSmRef), *sums = sm.floats(kSmSum), *inverse = sm.floats(kSmInverse);
+    int32_t *top = reinterpret_cast<int32_t *>(sm.ptr + kSmTop);
+    uint64_t *path = reinterpret_cast<uint64_t *>(sm.ptr + kSmPath), *cmp_path = path + kGroupOctets;
+    int32_t *length = reinterpret_cast<int32_t *>(cmp_path + kGroupOctets);
+    const uint32_t per_token = p.a.heads / kOctet;
+    uint32_t phase = 0, t = 0, vote = 0;
+    if (key < kGroupRows) top[key] = INT32_MIN;
+
+    Items it;
+    uint32_t items = 0;
+    for (bool more = it.first(p); more; more = it.advance(p), ++items) {
+        const uint32_t octets = (uint32_t)it.g.octets;
+        float sink = 0.f;
+        if (key < kGroupRows) {
+            const bool there = key < octets * kOctet;
+            const uint64_t row = (uint64_t)it.g.first_octet * kOctet + key;
+            const float *alphas = reinterpret_cast<const float *>(p.at(p.s.alphas));
+            alpha[key] = there ? __ldcg(alphas + row) : 0.f;
+            alpha[64 + key] = there && p.s.kinds == 2u ? __ldcg(alphas + (uint64_t)p.s.octets * kOctet + row) : 0.f;
+            ref[key] = kNoKey;
+            if (there) sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
+        } else if (key < kGroupRows + kGroupOctets) {
+            const uint32_t o = key - kGroupRows;
+            uint64_t m = 0, c = 0;
+            if (o < octets) {
+                const uint32_t token = ((uint32_t)it.g.first_octet + o) / per_token;
+                m = reinterpret_cast<const uint64_t *>(p.a.paths)[token];
+                if (it.g.drafted < (int32_t)kTreeDraft) m &= (1ull << it.g.drafted) - 1ull;
+                if (p.a.cmpPaths) c = reinterpret_cast<const uint64_t *>(p.a.cmpPaths)[token];
+            }
+            path[o] = m;
+            cmp_path[o] = c;
+            length[o] = __popcll(m);
+        }
+        if (!softmax_sync(sm, phase)) return;
+        const uint32_t present = (1u << octets) - 1u;
+        const int32_t whole_rows = max(it.g.prefix, 0) / 128;
+        float row_sum[2] = {0.f, 0.f};                        // this warp's share of the denominators of rows lane and 32 + lane
+
+        for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
+            const bool ori = j < (uint32_t)it.g.ori_tiles;
+            const float *scale = alpha + (ori ? 0 : 64);
+            const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
+            // ---- which octets see this key, and how often (a bias of log2 of the count)
+            uint32_t sees = 0;
+            float bias[LISTED ? 8 : 1];
+            uint4 count = make_uint4(0, 0, 0, 0);
+            if (LISTED && !ori) {
+                const uint32_t entry = (j - (uint32_t)it.g.ori_tiles) * kTile + key;
+                const uint64_t at = (uint64_t)it.g.first_octet * p.a.topk + entry;
+                if (entry < (uint32_t)it.g.cmp_rows && __ldcg(reinterpret_cast<const int32_t *>(p.at(p.s.rows)) + at) >= 0)
+                    count = __ldcg(reinterpret_cast<const uint4 *>(p.at(p.s.counts)) + at);
+            }
+            if (LISTED) {
+                const uint32_t words[4] = {count.x, count.y, count.z, count.w};
+#pragma unroll
+                for (uint32_t o = 0; o < 8; ++o) {
+                    const uint32_t n = (words[o / 2u] >> ((o & 1u) * 16u)) & 0xffffu;
+                    if (n) sees |= 1u << o;
+                    bias[o] = n > 1u ? log2f((float)n) : 0.f;
+                }
+            }
+            if (!LISTED || ori) {
+                if (!walk_wait<0>(sm, kBarKeyFull + (4u * t) % kRing, ph)) return;      // the page mask comes with segment 0
+                if ((flags[kFlagPages + (t & 3u)] >> warp) & 1u) {
+                    const int32_t row = (ori ? window_page(it.g.prefix, p.a.window) * (int32_t)kTreePage + (int32_t)(j * kTile)
+                                             : (int32_t)((j - (uint32_t)it.g.ori_tiles) * kTile)) + (int32_t)key;
+                    if (ori) {
+                        const int32_t drafted = row - it.g.prefix;
+#pragma unroll
+                        for (uint32_t o = 0; o < 8; ++o) {
+                            const bool seen = drafted < 0 ? drafted + (int32_t)p.a.window >= length[o]
+                                                          : drafted < (int32_t)kTreeDraft && ((path[o] >> drafted) & 1ull);
+                            sees |= seen ? 1u << o : 0u;
+                        }
+                    } else if (row < whole_rows) {
+                        sees = 0xffu;
+                    } else if (row - whole_rows < (int32_t)kTreeDraft) {
+#pragma unroll
+                        for (uint32_t o = 0; o < 8; ++o) sees |= (uint32_t)((cmp_path[o] >> (row - whole_rows)) & 1ull) << o;
+                    }
+                }
+            }
+            sees &= present;
+            const bool all = __all_sync(0xffffffffu, sees == 0xffu) && !LISTED;
+
+            // ---- logits against the references
+            if (!walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
+            tc_fence_after();
+            float x[kGroupRows];
+            auto logits = [&](bool absolute) {
+#pragma unroll
+                for (uint32_t c = 0; c < 4; ++c) {
+                    uint32_t hi[16], lo[16];
+                    tmem_ld16(tmem_lane + kColScore + buf * kCodeRows + c * 16u, hi);
+                    tmem_ld16(tmem_lane + kColScore + buf * kCodeRows + kGroupRows + c * 16u, lo);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        const float4 a = reinterpret_cast<const float4 *>(scale)[c * 4u + q], m = reinterpret_cast<const float4 *>(ref)[c * 4u + q];
+                        const float as[4] = {a.x, a.y, a.z, a.w}, ms[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint32_t r = q * 4u + i;
+                            float off = absolute ? 0.f : -ms[i];
+                            if (LISTED) off += bias[(c * 16u + r) / kOctet];
+                            x[c * 16u + r] = fmaf((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), as[i], off);
+                        }
+                    }
+                }
+                if (!all) {
+#pragma unroll
+                    for (uint32_t r = 0; r < kGroupRows; ++r) x[r] = (sees >> (r / kOctet)) & 1u ? x[r] : -INFINITY;
+                }
+            };
+            logits(false);
+            float most = x[0];
+#pragma unroll
+            for (uint32_t r = 1; r < kGroupRows; ++r) most = fmaxf(most, x[r]);
+            if (most > 0.f) flags[kFlagVote + vote] = 1;
+            if (!softmax_sync(sm, phase)) return;
+            const bool moved = flags[kFlagVote + vote] != 0;
+            vote = vote == 2u ? 0u : vote + 1u;
+            if (key == 0) {
+                // the slot after next was last read before the barrier just passed, and is set behind the next one
+                flags[kFlagVote + (vote == 2u ? 0u : vote + 1u)] = 0;
+                flags[kFlagRescale + buf] = moved;
+            }
+            if (moved) {
+                // exact row maxima: integers in float order, over the lanes by reduction, over the warps by atomicMax
+                logits(true);
+                int32_t high[2] = {INT32_MIN, INT32_MIN};
+#pragma unroll
+                for (uint32_t r = 0; r < kGroupRows; ++r) {
+                    const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x[r])));
+                    if (lane == (r & 31u)) high[r >> 5] = v;
+                }
+                atomicMax(top + lane, high[0]);
+                atomicMax(top + 32 + lane, high[1]);
+                if (!softmax_sync(sm, phase)) return;
+                if (key < kGroupRows) {
+                    const float highest = __int_as_float(ordered(top[key])), old = ref[key];
+                    float now = old, factor = 1.f;
+                    if (highest > old - 1.f) {                // the margin covers the rounding of x; a NaN moves nothing
+                        now = highest + kHeadroom;
+                        factor = exp2_approx(old - now);
+                    }
+                    top[key] = INT32_MIN;
+                    ref[key] = now;
+                    sm.floats(kSmFactor)[buf * kGroupRows + key] = factor;
+                }
+                if (!softmax_sync(sm, phase)) return;
+                row_sum[0] *= sm.floats(kSmFactor)[buf * kGroupRows + lane];
+                row_sum[1] *= sm.floats(kSmFactor)[buf * kGroupRows + 32u + lane];
+                logits(false);
+            }
+            tc_fence_before();
+            mbar_arrive(sm.bar(kBarScoreFree + buf));
+
+            // ---- weights as codes
+            if (t >= 2u && !walk_wait<0>(sm, kBarWeightFree + buf, ph ^ 1u)) return;
+            char *weights = sm.ptr + kSmWeight + buf * kSeg + key * 128u;
+            uint32_t total[2] = {0, 0};
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (uint32_t q = 0; q < 4; ++q) {
+                    uint32_t d[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t r = c * 16u + q * 4u + i;
+                        d[i] = __float_as_uint(__fmaf_rn(exp2_approx(x[r]), kWeightSteps, 8388736.f));     // 2^23 + 128 + code
+                        const uint32_t s = __reduce_add_sync(0xffffffffu, d[i]);
+                        if (lane == (r & 31u)) total[r >> 5] = s - 32u * kCodeBias;
+                    }
+                    hi[q] = __byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410);
+                    lo[q] = __byte_perm(__byte_perm(d[0], d[1], 0x0040), __byte_perm(d[2], d[3], 0x0040), 0x5410) ^ 0x80808080u;
+                }
+                *reinterpret_cast<uint4 *>(weights + ((c ^ (key & 7u)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4 *>(weights + (((4u + c) ^ (key & 7u)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(sm.bar(kBarWeightReady + buf));
+            row_sum[0] += (float)total[0];
+            row_sum[1] += (float)total[1];
+        }
+
+        // ---- denominators, the warps' shares added in warp order
+#pragma unroll 1
+        for (uint32_t w = 0; w < 4; ++w) {
+            if (warp == w) {
+                sums[lane] = w ? sums[lane] + row_sum[0] : row_sum[0];
+                sums[32 + lane] = w ? sums[32 + lane] + row_sum[1] : row_sum[1];
+            }
+            if (!softmax_sync(sm, phase)) return;
+        }
+        if (!walk_wait<0>(sm, kBarDoneFree, (items & 1u) ^ 1u)) return;
+        if (key < octets * kOctet) {
+            float l = sums[key];
+            if (alpha[key] != alpha[key]) l = alpha[key];     // a query row that is not finite
+            const float m = ref[key];
+            if (it.whole()) {
+                const float sink2 = sink * kLog2e, at = fmaxf(m, sink2), own = exp2_approx(m - at);
+                const float all_sum = l * own + (sink == -INFINITY ? 0.f : kWeightSteps * exp2_approx(sink2 - at));
+                inverse[key] = all_sum == 0.f ? 0.f : own / all_sum;
+                if (p.a.lse)
+                    reinterpret_cast<float *>(p.a.lse)[(uint64_t)it.g.first_octet * kOctet + key] =
+                        all_sum == 0.f ? -INFINITY : (at + log2f(all_sum * (1.f / kWeightSteps))) * kLn2;
+            } else {
+                float *mine = reinterpret_cast<float *>(p.at(p.s.partials)) + (uint64_t)it.partial() * kPartial + kGroupRows * kDim;
+                mine[key] = l;
+                mine[kGroupRows + key] = m;
+            }
+        }
+        mbar_arrive(sm.bar(kBarDone));
+    }
+}
+
+// ------------------------------------------------------------------ walk: accumulate (warps 4-11)
+// Thread = channel of each 128-channel block, rows 32 h .. 32 h + 31: 128 running sums in registers.  The
+// integers of a block are read, joined, scaled and added while the tensor core fills the other block.
+__device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
+{
+    const uint32_t index = threadIdx.x - kWarpAccumulate * 32u, h = index >> 7, channel = index & 127u, warp = channel >> 5;
+    const uint32_t tmem_lane = tmem + ((warp * 32u) << 16) + kColOut + h * 32u;
+    Items it;
+    uint32_t t = 0, items = 0;
+    for (bool more = it.first(p); more; more = it.advance(p), ++items) {
+        float acc[4][32];
+#pragma unroll
+        for (int block = 0; block < 4; ++block)
+#pragma unroll
+            for (int r = 0; r < 32; ++r) acc[block][r] = 0.f;
+        for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
+            const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
+            if (!walk_wait<1>(sm, kBarWeightReady + buf, ph)) return;
+            if (sm.flags()[kFlagRescale + buf]) {
+                const float4 *factor = reinterpret_cast<const float4 *>(sm.ptr + kSmFactor) + buf * 16u + h * 8u;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 f = factor[q];
+#pragma unroll
+                    for (int block = 0; block < 4; ++block) {
+                        acc[block][4 * q] *= f.x; acc[block][4 * q + 1] *= f.y;
+                        acc[block][4 * q + 2] *= f.z; acc[block][4 * q + 3] *= f.w;
+                    }
+                }
+            }
+            const float *scale = reinterpret_cast<const float *>(j < (uint32_t)it.g.ori_tiles ? p.a.oriScale : p.a.cmpScale) + channel;
+#pragma unroll
+            for (uint32_t block = 0; block < 4; ++block) {
+                const float s = __ldg(scale + block * 128u);
+                const uint32_t half = block & 1u;
+                if (!walk_wait<1>(sm, kBarOutFull + half, (block >> 1) & 1u)) return;
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t c = 0; c < 4; ++c) {
+                    uint32_t hi[8], lo[8];
+                    tmem_ld8(tmem_lane + half * kCodeRows + c * 8u, hi);
+                    tmem_ld8(tmem_lane + half * kCodeRows + kGroupRows + c * 8u, lo);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        acc[block][c * 8u + i] = fmaf((float)((int32_t)hi[i] * 256 + (int32_t)lo[i]), s, acc[block][c * 8u + i]);
+                }
+                tc_fence_before();
+                mbar_arrive(sm.bar(kBarOutFree + half));
+            }
+        }
+        if (!walk_wait<1>(sm, kBarDone, items & 1u)) return;
+        const uint32_t rows = (uint32_t)it.g.octets * kOctet;
+        if (it.whole()) {
+            const float *inverse = sm.floats(kSmInverse) + h * 32u;
+            __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.a.out) + ((uint64_t)it.g.first_octet * kOctet + h * 32u) * kDim + channel;
+#pragma unroll
+            for (uint32_t r = 0; r < 32; ++r) {
+                if (h * 32u + r < rows) {
+                    const float f = inverse[r];
+#pragma unroll
+                    for (uint32_t block = 0; block < 4; ++block) out[r * kDim + block * 128u] = __float2bfloat16_rn(acc[block][r] * f);
+                }
+            }
+        } else {
+            float *mine = reinterpret_cast<float *>(p.at(p.s.partials)) + (uint64_t)it.partial() * kPartial + h * 32u * kDim + channel;
+#pragma unroll
+            for (uint32_t r = 0; r < 32; ++r)
+                if (h * 32u + r < rows)
+#pragma unroll
+                    for (uint32_t block = 0; block < 4; ++block) mine[r * kDim + block * 128u] = acc[block][r];
+        }
+        mbar_arrive(sm.bar(kBarDoneFree));
+    }
+}
+
+template <bool LISTED>
+__global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid_constant__ Tree p, const __grid_constant__ CUtensorMap ori_map,
+                                                                     const __grid_constant__ CUtensorMap cmp_map,
+                                                                     const __grid_constant__ CUtensorMap row_map, const uint32_t gather)
+{
+    extern __shared__ __align__(1024) char smem_walk[];
+    WalkShared sm;
+    sm.base = smem_addr(smem_walk);
+    sm.ptr = smem_walk;
+    const uint32_t warp = threadIdx.x >> 5;
+    volatile uint32_t *flags = sm.flags();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kRing; ++i) { mbar_init(sm.bar(kBarKeyFull + i), 1); mbar_init(sm.bar(kBarKeyEmpty + i), 1); }
+        mbar_init(sm.bar(kBarQueryFull), 1);
+        mbar_init(sm.bar(kBarQueryEmpty), 1);
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(sm.bar(kBarScoreFull + i), 1); mbar_init(sm.bar(kBarScoreFree + i), 128);
+            mbar_init(sm.bar(kBarWeightReady + i), 128); mbar_init(sm.bar(kBarWeightFree + i), 1);
+            mbar_init(sm.bar(kBarOutFull + i), 1); mbar_init(sm.bar(kBarOutFree + i), 256);
+        }
+        mbar_init(sm.bar(kBarSync), 128);
+        mbar_init(sm.bar(kBarDone), 128);
+        mbar_init(sm.bar(kBarDoneFree), 256);
+        for (uint32_t i = 0; i < 12; ++i) if (i != kFlagTmem) flags[i] = 0;
+        fence_mbar_init();
+    }
+    if (warp == kWarpIssue) {
+        tmem_alloc(sm.base + kSmFlags + 4u * kFlagTmem, kTmemAll);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = flags[kFlagTmem];
+    grid_dependency_launch_dependents();
+    grid_dependency_wait();
+
+    if (warp < kWarpAccumulate) {
+        softmax<LISTED>(p, sm, tmem);
+    } else if (warp < kWarpIssue) {
+        registers_acquire<kRegsAccumulate>();
+        accumulate(p, sm, tmem);
+    } else {
+        registers_release<kRegsIssue>();
+        if (warp == kWarpIssue) issue(p, sm, tmem);
+        else produce<LISTED>(p, sm, warp - kWarpProduce, &ori_map, &cmp_map, &row_map, gather != 0);
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (flags[kFlagAbort]) {
+        // A wait ran out: copies and products already issued may still land in this block's memory, so it
+        // stays for far longer than they can take before it gives that memory up.
+        if (threadIdx.x == 0) p.head()[0] = kStatusWaitTimeout;
+        for (uint32_t i = 0; i < 200u; ++i) __nanosleep(1000u);
+        __syncthreads();
+    }
+    if (warp == kWarpIssue) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemAll);
+    }
+}
+
+// ------------------------------------------------------------------ merge
+// Block (i, o): octet o of the group that cut i is the first to fall into.  Pieces are joined in piece
+// order: M = max of the references and the sink, out = sum O 2^(ref - M) / (sum l 2^(ref - M) + sink).
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const __grid_constant__ Tree p)
+{
+    grid_dependency_launch_dependents();
+    grid_dependency_wait();
+    const uint2 *cuts = reinterpret_cast<const uint2 *>(p.at(p.s.cuts));
+    const uint32_t i = blockIdx.x + 1u, octet = blockIdx.y;
+    const uint2 cut = __ldcg(cuts + i);
+    if (cut.y == 0 || cut.x >= p.s.slots) return;
+    const uint2 before = __ldcg(cuts + i - 1u);
+    if (before.x == cut.x && before.y != 0) return;           // an earlier cut has the group
+    const Group g = p.groups()[cut.x];
+    if (octet >= (uint32_t)g.octets) return;
+    uint32_t pieces = 2;
+    while (i + pieces - 1u < p.grid) {
+        const uint2 next = __ldcg(cuts + i + pieces - 1u);
+        if (next.x != cut.x || next.y == 0) break;
+        ++pieces;
+    }
+    const float *partials = reinterpret_cast<const float *>(p.at(p.s.partials));
+    const uint32_t row = octet * kOctet + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
+    auto piece = [&](uint32_t q) { return partials + (uint64_t)(q == 0 ? 2u * (i - 1u) + 1u : 2u * (i - 1u + q)) * kPartial; };
+    const uint64_t global_row = (uint64_t)g.first_octet * kOctet + row;
+    const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + global_row % p.a.heads), sink2 = sink * kLog2e;
+    float at = sink2;
+#pragma unroll 4
+    for (uint32_t q = 0; q < pieces; ++q) at = fmaxf(at, __ldcg(piece(q) + kGroupRows * kDim + kGroupRows + row));
+    float total = sink == -INFINITY ? 0.f : kWeightSteps * exp2_approx(sink2 - at);
+    float acc[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] = 0.f;
+#pragma unroll 2
+    for (uint32_t q = 0; q < pieces; ++q) {
+        const float *src = piece(q);
+        const float f = exp2_approx(__ldcg(src + kGroupRows * kDim + kGroupRows + row) - at);
+        total = fmaf(__ldcg(src + kGroupRows * kDim + row), f, total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + row * kDim) + k * 32 + lane);
+            acc[4 * k] = fmaf(v.x, f, acc[4 * k]); acc[4 * k + 1] = fmaf(v.y, f, acc[4 * k + 1]);
+            acc[4 * k + 2] = fmaf(v.z, f, acc[4 * k + 2]); acc[4 * k + 3] = fmaf(v.w, f, acc[4 * k + 3]);
+        }
+    }
+    const float inverse = total == 0.f ? 0.f : 1.f / total;
+    __nv_bfloat162 *out = reinterpret_cast<__nv_bfloat162 *>(reinterpret_cast<__nv_bfloat16 *>(p.a.out) + global_row * kDim);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        out[(k * 32 + lane) * 2] = __floats2bfloat162_rn(acc[4 * k] * inverse, acc[4 * k + 1] * inverse);
+        out[(k * 32 + lane) * 2 + 1] = __floats2bfloat162_rn(acc[4 * k + 2] * inverse, acc[4 * k + 3] * inverse);
+    }
+    if (p.a.lse && lane == 0)
+        reinterpret_cast<float *>(p.a.lse)[global_row] = total == 0.f ? -INFINITY : (at + log2f(total * (1.f / kWeightSteps))) * kLn2;
+}
+
+// ------------------------------------------------------------------ host
+using TreeEncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                     const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+TreeEncodeTiled tree_encode_tiled()
+{
+    static std::atomic<void *> cached{nullptr};
+    void *fn = cached.load(std::memory_order_acquire);
+    if (fn == nullptr) {
+        cudaDriverEntryPointQueryResult status;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &status) != cudaSuccess ||
+            status != cudaDriverEntryPointSuccess)
+            return nullptr;
+        cached.store(fn, std::memory_order_release);
+    }
+    return reinterpret_cast<TreeEncodeTiled>(fn);
+}
+
+// Pages as [pages, 32 rows, 512 bytes], boxes of `rows` rows x 128 bytes; or, with rows = 0, the whole pool as rows of
+// 512 bytes for gathers (ids beyond it read as zeros).
+bool tree_map(CUtensorMap *map, uint64_t base, uint64_t stride, uint32_t pages, uint32_t rows)
+{
+    const TreeEncodeTiled encode = tree_encode_tiled();
+    if (encode == nullptr) return false;
+    const cuuint32_t ones[3] = {1, 1, 1};
+    if (rows == 0) {
+        const cuuint64_t dims[2] = {kDim, 0x7ffffff0ull}, strides[1] = {kDim};
+        const cuuint32_t box[2] = {128, 1};
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, reinterpret_cast<void *>(base), dims, strides, box, ones,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    const cuuint64_t dims[3] = {kDim, kTreePage, pages}, strides[2] = {kDim, stride};
+    const cuuint32_t box[3] = {128, rows, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, reinterpret_cast<void *>(base), dims, strides, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class... Params, class... Args>
+cudaError_t tree_launch(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream, const Args &...args)
+{
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = programmatic_launch_enabled() ? 1u : 0u;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+// The opt-in to large dynamic shared memory, once per device and kernel.
+template <class Kernel>
+cudaError_t tree_opt_in(Kernel kernel, uint32_t smem, std::atomic<uint64_t> &configured)
+{
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device >= 0 && device < kMaxDevices ? 1ull << device : 0ull;
+    if (bit && (configured.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) configured.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+constexpr uint32_t kUnionSmem = 2u * (kUnionRows / 32u) * 4u + 8192u * 16u;      // bitmap, ranks, counts of 8 x 1024 entries
+
+int tree_launch_all(const TreeAttentionArgs &a, cudaStream_t stream, int sms)
+{
+    Tree p;
+    p.a = a;
+    p.s = tree_space(a.tokens, a.heads, a.batch, a.ratio, a.topk);
+    p.grid = (uint32_t)sms < split::kMaxCtas ? (uint32_t)sms : split::kMaxCtas;
+    const bool listed = a.ratio == 4u;
+    const bool gather = a.cmpStride % kDim == 0 && (uint64_t)a.cmpPages * (a.cmpStride / kDim) < 0x7ffffff0ull;
+    CUtensorMap ori_map, cmp_map, row_map;
+    if (!tree_map(&ori_map, a.ori, a.oriStride, a.oriPages, kTreePage) || !tree_map(&cmp_map, a.cmp, a.cmpStride, a.cmpPages, kTreePage) ||
+        !tree_map(&row_map, a.cmp, a.cmpStride, a.cmpPages, listed && gather ? 0u : 1u))
+        return SHAREDKV_EINVAL;
+    static std::atomic<uint64_t> walk_pages{0}, walk_rows{0}, unions{0};
+    cudaError_t e = tree_launch(tree_encode_kernel, dim3(p.s.octets), kEncodeThreads, 0u, stream, p);
+    if (e == cudaSuccess && listed) {
+        e = tree_opt_in(tree_union_kernel, kUnionSmem, unions);
+        if (e == cudaSuccess) e = tree_launch(tree_union_kernel, dim3(p.s.slots), kUnionThreads, kUnionSmem, stream, p);
+        if (e == cudaSuccess) e = tree_opt_in(tree_walk_kernel<true>, kWalkSmem, walk_rows);
+        if (e == cudaSuccess) e = tree_launch(tree_walk_kernel<true>, dim3(p.grid), kWalkThreads, kWalkSmem, stream, p, ori_map, cmp_map, row_map, (uint32_t)gather);
+    } else if (e == cudaSuccess) {
+        e = tree_opt_in(tree_walk_kernel<false>, kWalkSmem, walk_pages);
+        if (e == cudaSuccess) e = tree_launch(tree_walk_kernel<false>, dim3(p.grid), kWalkThreads, kWalkSmem, stream, p, ori_map, cmp_map, row_map, 0u);
+    }
+    if (e == cudaSuccess && p.grid > 1u) e = tree_launch(tree_merge_kernel, dim3(p.grid - 1u, kGroupOctets), kMergeThreads, 0u, stream, p);
+    return (int)e;
 }
 
 }  // namespace
 
-uint64_t tree_workspace_bytes(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) { return 256; }
+uint64_t tree_workspace_bytes(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk)
+{
+    return tree_space(tokens, heads, batch, ratio, topk).bytes;
+}
 
 int tree_attention(const TreeAttentionArgs *args, cudaStream_t stream)
 {
@@ -106,7 +1219,7 @@ int tree_attention(const TreeAttentionArgs *args, cudaStream_t stream)
     TreeAttentionArgs a = *args;
     if (a.tokens == 0 || a.batch == 0) return SHAREDKV_OK;
     if (a.ratio != 1u && a.ratio != 4u && a.ratio != 128u) return SHAREDKV_EINVAL;
-    if (a.heads == 0 || a.heads % kTreeHeads || a.heads > 128u || a.window == 0 || a.window > 65536u) return SHAREDKV_EINVAL;
+    if (a.heads == 0 || a.heads % kOctet || a.heads > 128u || a.window == 0 || a.window > 65536u) return SHAREDKV_EINVAL;
     if (a.ratio == 1u) {
         // no compressed kind: its fields alias the original cache so that nothing in the kernel is null
         a.cmp = a.ori; a.cmpScale = a.oriScale; a.cmpTable = a.oriTable; a.cmpStride = a.oriStride;
@@ -125,16 +1238,9 @@ int tree_attention(const TreeAttentionArgs *args, cudaStream_t stream)
     if (!a.oriTableWidth || !a.cmpTableWidth || !a.oriPages || !a.cmpPages || a.oriPages >= (1u << 26) || a.cmpPages >= (1u << 26) ||
         a.oriTableWidth >= (1u << 26) || a.cmpTableWidth >= (1u << 26))
         return SHAREDKV_EINVAL;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(a.tokens, a.heads / kTreeHeads);
-    config.blockDim = dim3(kTreeThreads);
-    config.stream = stream;
-    cudaLaunchAttribute attribute[1];
-    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute[0].val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = attribute;
-    config.numAttrs = programmatic_launch_enabled() ? 1u : 0u;
-    return (int)cudaLaunchKernelEx(&config, tree_simple_kernel, a);
+    const int sms = device_sm_count();
+    if (sms <= 0) return (int)cudaErrorInvalidDevice;
+    return tree_launch_all(a, stream, sms);
 }
 
 }  // namespace sharedkv

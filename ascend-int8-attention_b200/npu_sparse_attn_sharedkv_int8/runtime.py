@@ -50,6 +50,7 @@ def _library():
         getattr(lib, name).argtypes, getattr(lib, name).restype = [], u32
     lib.sharedkv_tree_workspace_bytes.argtypes, lib.sharedkv_tree_workspace_bytes.restype = [u32] * 5, u64
     lib.sharedkv_tree_attention.argtypes, lib.sharedkv_tree_attention.restype = [u64, i32, ptr], ctypes.c_int
+    lib.sharedkv_tree_status.argtypes, lib.sharedkv_tree_status.restype = [ptr, ptr], ctypes.c_int
     lib.sharedkv_page_workspace_bytes.argtypes, lib.sharedkv_page_workspace_bytes.restype = [u32, u32], u64
     lib.sharedkv_page.argtypes, lib.sharedkv_page.restype = [u64, u32, u64, u64, u32, i32, ptr], ctypes.c_int
     lib.sharedkv_page_status.argtypes, lib.sharedkv_page_status.restype = [ptr, ptr], ctypes.c_int

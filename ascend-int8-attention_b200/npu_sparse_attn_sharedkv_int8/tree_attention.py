@@ -93,9 +93,12 @@ class PreparedTreeAttention:
             lse = torch.empty((tokens, heads), dtype=torch.float32, device=device)
         need = self.kernels.lib.sharedkv_tree_workspace_bytes(tokens, heads, args.batch, case.ratio, args.topk)
         allocate = scratch_allocator or (lambda name, shape, dtype, where: torch.empty(shape, dtype=dtype, device=where))
-        self.workspace = allocate("tree_workspace", (max(need, 256),), torch.uint8, device)
+        self.workspace = allocate("tree_workspace", (max(need, 1024),), torch.uint8, device)
         _require(self.workspace.data_ptr() % 256 == 0, "Attention workspace must be 256-byte aligned")
         args.workspace = self.workspace.data_ptr()
+        # arrival counters and status start at zero and every launch leaves them so
+        with torch.cuda.device(device):
+            check(self.kernels.lib.sharedkv_workspace_init(args.workspace, current_stream(device.index)), "workspace init")
         self.argument_address = ctypes.addressof(args)
         self._rebind_same_geometry(case, paths, cmp_paths=cmp_paths, output=out, lse_output=lse)
 
@@ -121,6 +124,12 @@ class PreparedTreeAttention:
             check(self.kernels.lib.sharedkv_tree_attention(self.argument_address, self.device_index, current_stream(self.device_index)),
                   "tree attention launch")
         return self.out
+
+    def status(self):
+        """Synchronises the current stream; raises RuntimeError if a wait inside a launch of this operator ran
+        out (its results are then invalid).  Diagnostic only."""
+        with torch.cuda.device(self.case.q.device):
+            check(self.kernels.lib.sharedkv_tree_status(self.args.workspace, current_stream(self.device_index)), "tree attention kernel")
 
 
 __all__ = ["DIM", "DRAFT_ROWS", "PreparedTreeAttention", "path_masks"]

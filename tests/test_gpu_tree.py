@@ -30,6 +30,7 @@ def prepared(made, stride=None, offset=0, **more):
 
 
 def check(op, made, label=""):
+    op.status()
     want, want_lse, bound, lse_bound = expected(*made)
     got, got_lse = op.out.cpu().double(), op.lse.cpu().double()
     worst = ((got - want).abs() - bound).max()
