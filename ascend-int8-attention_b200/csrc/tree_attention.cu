@@ -46,13 +46,13 @@ constexpr uint32_t kCodeRows = 2 * kGroupRows;               // hi plane, then l
 constexpr uint32_t kTile = 128;                              // keys of a tile
 constexpr uint32_t kSeg = kTile * 128;                       // one 128-channel segment of a tile (or of the query codes): 16 KB
 constexpr uint32_t kRing = 8;                                // segments in flight: two tiles
-constexpr uint32_t kWalkThreads = 512;
+constexpr uint32_t kWalkThreads = 640;
 constexpr uint32_t kEncodeThreads = 256, kUnionThreads = 1024, kMergeThreads = 256;
-constexpr uint32_t kWarpAccumulate = 4, kWarpIssue = 12, kWarpProduce = 13, kProducers = 3;
-// Registers: launched with 128 per thread; accumulate (two warps of every SM partition) grows to hold
-// 128 running sums a thread, the issuer and the producers shrink.  168 + 168 + 128 + 48 = 4 x 128.
-constexpr uint32_t kRegsAccumulate = 168, kRegsIssue = 48;
-static_assert(2 * kRegsAccumulate + 128 + kRegsIssue <= 4 * 128, "register shares exceed the launch allocation");
+constexpr uint32_t kWarpAccumulate = 8, kWarpIssue = 16, kWarpProduce = 17, kProducers = 3;
+// Registers: launched with 96 per thread; accumulate (two warps of every SM partition) grows to hold
+// 128 running sums a thread, the others shrink.
+constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 56, kRegsAccumulate = 168, kRegsIssue = 32;
+static_assert(2 * kRegsSoftmax + 2 * kRegsAccumulate + kRegsIssue <= 5 * kRegsLaunch, "register shares exceed the launch allocation");
 constexpr float kWeightSteps = 32639.f;                      // 127 * 256 + 127: the largest weight code
 constexpr uint32_t kCodeBias = 0x4b000080u;                  // bits of 2^23 + 128
 constexpr float kNoKey = -1e30f;                             // reference of a row that has met no key
@@ -74,15 +74,15 @@ constexpr uint32_t kSmFactor = kSmTop + 256;                 // FP32 [2][64] res
 constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [64] denominators
 constexpr uint32_t kSmInverse = kSmSum + 256;                // FP32 [64]
 constexpr uint32_t kSmPath = kSmInverse + 256;               // UINT64 [8] paths, UINT64 [8] compressed paths, INT32 [8] path lengths
-constexpr uint32_t kSmFlags = kSmPath + 160;                 // rescale [2], vote [3], page masks [4], tmem base, abort
-constexpr uint32_t kSmBars = kSmFlags + 48;
+constexpr uint32_t kSmFlags = kSmPath + 160;                 // rescale [2 tiles][2 halves], vote [2 halves][3], page masks [4], tmem base, abort
+constexpr uint32_t kSmBars = kSmFlags + 64;
 constexpr uint32_t kBarKeyFull = 0, kBarKeyEmpty = 8, kBarQueryFull = 16, kBarQueryEmpty = 17, kBarScoreFull = 18, kBarScoreFree = 20,
-                   kBarWeightReady = 22, kBarWeightFree = 24, kBarOutFull = 26, kBarOutFree = 28, kBarSync = 30, kBarDone = 31,
-                   kBarDoneFree = 32, kTreeBars = 33;
+                   kBarWeightReady = 22, kBarWeightFree = 24, kBarOutFull = 26, kBarOutFree = 28, kBarSync = 30, kBarDone = 32,
+                   kBarDoneFree = 33, kTreeBars = 34;
 constexpr uint32_t kWalkSmem = kSmBars + 8 * kTreeBars;
 static_assert(kWalkSmem <= 232448, "dynamic shared memory limit of sm_100");
 static_assert(kSmPath % 8 == 0 && kSmBars % 8 == 0, "64-bit words");
-constexpr uint32_t kFlagRescale = 0, kFlagVote = 2, kFlagPages = 5, kFlagTmem = 9, kFlagAbort = 10;
+constexpr uint32_t kFlagRescale = 0, kFlagVote = 4, kFlagPages = 10, kFlagTmem = 14, kFlagAbort = 15;
 constexpr uint32_t kTmemAll = 512, kColScore = 0, kColOut = 256;      // two score tiles, two 128-channel blocks of O
 
 struct Group {
@@ -224,20 +224,22 @@ __device__ bool last_block(const Tree &p, uint32_t blocks)
 }
 
 // ------------------------------------------------------------------ encode
-// One block per octet, a warp per head: lane l owns channels 16 l .. 16 l + 15, one 16-byte chunk of a code
+// A block takes octets in turn, a warp per head: lane l owns channels 16 l .. 16 l + 15, one 16-byte chunk of a code
 // row.  Codes go out as the walk's B operand wants them: [kind][segment][plane][octet] blocks of 8 rows x
 // 128 bytes, swizzled, so that a group's rows of a plane are one contiguous copy.
-__device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_t octet, uint32_t row, const float (&q)[16])
+__device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_t octet, uint32_t row, const float (&q)[16], const float *sm_scale)
 {
     const uint32_t lane = threadIdx.x & 31u;
-    const float *scale = reinterpret_cast<const float *>(kind ? p.a.cmpScale : p.a.oriScale) + lane * 16u;
+    const float4 *scale = reinterpret_cast<const float4 *>(sm_scale + kind * kDim) + lane;      // [4][32 lanes]: no bank conflicts
     float f[16];
     uint32_t top = 0;                                         // largest |f| as an integer: a NaN or an infinity wins
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        f[i] = q[i] * __ldg(scale + i);
-        top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+    for (int i = 0; i < 4; ++i) {
+        const float4 v = scale[i * 32];
+        f[4 * i] = q[4 * i] * v.x; f[4 * i + 1] = q[4 * i + 1] * v.y; f[4 * i + 2] = q[4 * i + 2] * v.z; f[4 * i + 3] = q[4 * i + 3] * v.w;
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
     top = __reduce_max_sync(0xffffffffu, top);
     const bool finite = top < 0x7f800000u;
     const float alpha = fmaxf(__uint_as_float(top) * (float)(1.0 / 127), 1e-30f), rcp = __frcp_rn(alpha);
@@ -267,13 +269,22 @@ __device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_
 __global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __grid_constant__ Tree p)
 {
     __shared__ uint32_t shared_live;
+    __shared__ __align__(16) float sm_scale[2 * kDim];        // channel 16 l + 4 i + e of a kind at 128 i + 4 l + e
     grid_dependency_launch_dependents();
     grid_dependency_wait();
-    const uint32_t lane = threadIdx.x & 31u, row = threadIdx.x >> 5, octet = blockIdx.x, per_token = p.a.heads / kOctet;
+    const uint32_t lane = threadIdx.x & 31u, row = threadIdx.x >> 5, per_token = p.a.heads / kOctet;
     const int32_t *cu = p.cu();
-    const uint32_t token = octet / per_token;
-    const uint4 *src = reinterpret_cast<const uint4 *>(p.a.q + ((uint64_t)octet * kOctet + row) * (kDim * 2u)) + lane * 2u;
-    const uint4 raw[2] = {src[0], src[1]};                    // in flight while the block finds out whose row it is
+    auto fetch = [&](uint32_t octet, uint4 (&raw)[2]) {
+        const uint4 *src = reinterpret_cast<const uint4 *>(p.a.q + ((uint64_t)octet * kOctet + row) * (kDim * 2u)) + lane * 2u;
+        raw[0] = src[0];
+        raw[1] = src[1];
+    };
+    uint4 raw[2];
+    fetch(blockIdx.x, raw);                                   // in flight while the block finds out what is live
+    for (uint32_t i = threadIdx.x; i < p.s.kinds * kDim; i += kEncodeThreads) {
+        const uint32_t c = i % kDim;
+        sm_scale[i / kDim * kDim + (c >> 2 & 3u) * 128u + (c >> 4) * 4u + (c & 3u)] = __ldg(reinterpret_cast<const float *>(i < kDim ? p.a.oriScale : p.a.cmpScale) + c);
+    }
     const uint32_t live = live_requests(p, &shared_live);
     const uint32_t live_tokens = split::live_token_count(live ? cu[live] : 0, p.a.tokens);
     // slots of no group: the empty ones between requests, and those behind the last
@@ -306,18 +317,22 @@ __global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __gri
         }
         p.groups()[i] = g;
     }
-    if (token >= live_tokens || (int32_t)token < cu[0]) {
-        const uint64_t at = ((uint64_t)octet * kOctet + row) * kDim;
-        uint4 *out = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.a.out) + at) + lane * 2u;
-        out[0] = out[1] = make_uint4(0, 0, 0, 0);
-        if (p.a.lse && lane == 0) reinterpret_cast<float *>(p.a.lse)[(uint64_t)octet * kOctet + row] = 0.f;
-    } else {
+    for (uint32_t octet = blockIdx.x; octet < p.s.octets; octet += gridDim.x) {
+        const uint32_t token = octet / per_token;
+        if (token >= live_tokens || (int32_t)token < cu[0]) {
+            const uint64_t at = ((uint64_t)octet * kOctet + row) * kDim;
+            uint4 *out = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.a.out) + at) + lane * 2u;
+            out[0] = out[1] = make_uint4(0, 0, 0, 0);
+            if (p.a.lse && lane == 0) reinterpret_cast<float *>(p.a.lse)[(uint64_t)octet * kOctet + row] = 0.f;
+            continue;
+        }
+        if (octet != blockIdx.x) fetch(octet, raw);
         float q[16];
         const uint32_t *words = reinterpret_cast<const uint32_t *>(raw);
 #pragma unroll
         for (int i = 0; i < 8; ++i) { q[2 * i] = __uint_as_float(words[i] << 16); q[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u); }
 #pragma unroll 1
-        for (uint32_t kind = 0; kind < p.s.kinds; ++kind) encode_row(p, kind, octet, row, q);
+        for (uint32_t kind = 0; kind < p.s.kinds; ++kind) encode_row(p, kind, octet, row, q, sm_scale);
     }
     if (p.a.ratio != 4u && last_block(p, gridDim.x)) cut_tiles(p);
 }
@@ -668,14 +683,16 @@ __device__ void issue(const Tree &p, const WalkShared &sm, uint32_t tmem)
     if (t) output_product(t - 1u);
 }
 
-// ------------------------------------------------------------------ walk: softmax (warps 0-3)
-// Thread = key of the tile; it holds the key's 64 logits.  Sums over keys (the denominators) and, when a
-// logit exceeds its row's reference, maxima over keys are warp reductions of integers, whose
-// result does not depend on their order.
-__device__ __forceinline__ bool softmax_sync(const WalkShared &sm, uint32_t &phase)
+// ------------------------------------------------------------------ walk: softmax (warps 0-7)
+// Two halves of four warps; thread (half, key) has the key's logits of rows 32 half .. 32 half + 31, four
+// octets, which it takes one after the other straight from tensor memory into weight codes.  That some
+// logit lies above its reference shows in passing; then the octets concerned get new references (exact
+// maxima) and are done again.  Maxima and sums over keys are warp reductions of integers, whose result
+// does not depend on their order.
+__device__ __forceinline__ bool softmax_sync(const WalkShared &sm, uint32_t half, uint32_t &phase)
 {
-    mbar_arrive(sm.bar(kBarSync));
-    const bool ok = walk_wait<0>(sm, kBarSync, phase);
+    mbar_arrive(sm.bar(kBarSync + half));
+    const bool ok = walk_wait<0>(sm, kBarSync + half, phase);
     phase ^= 1u;
     return ok;
 }
@@ -691,150 +708,177 @@ __device__ __forceinline__ int32_t ordered(int32_t bits) { return bits ^ ((bits 
 template <bool LISTED>
 __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
 {
-    const uint32_t key = threadIdx.x, lane = key & 31u, warp = key >> 5;
-    const uint32_t tmem_lane = tmem + ((warp * 32u) << 16);
+    constexpr uint32_t kOctets = kGroupOctets / 2, kRows = kGroupRows / 2;         // of a half
+    const uint32_t half = threadIdx.x >> 7, key = threadIdx.x & 127u, lane = key & 31u, warp = key >> 5;
+    const uint32_t score = tmem + ((warp * 32u) << 16) + kColScore + half * kRows;
     volatile uint32_t *flags = sm.flags();
-    float *alpha = sm.floats(kSmAlpha), *ref = sm.floats(kSmRef), *sums = sm.floats(kSmSum), *inverse = sm.floats(kSmInverse);
-    int32_t *top = reinterpret_cast<int32_t *>(sm.ptr + kSmTop);
-    uint64_t *path = reinterpret_cast<uint64_t *>(sm.ptr + kSmPath), *cmp_path = path + kGroupOctets;
-    int32_t *length = reinterpret_cast<int32_t *>(cmp_path + kGroupOctets);
+    float *ref = sm.floats(kSmRef) + half * kRows, *sums = sm.floats(kSmSum) + half * kRows;
+    int32_t *top = reinterpret_cast<int32_t *>(sm.ptr + kSmTop) + half * kRows;
     const uint32_t per_token = p.a.heads / kOctet;
-    uint32_t phase = 0, t = 0, vote = 0;
-    if (key < kGroupRows) top[key] = INT32_MIN;
+    uint32_t phase = 0, t = 0, vote = kFlagVote + half * 3u;
+    if (key < kRows) top[key] = INT32_MIN;
 
     Items it;
     uint32_t items = 0;
     for (bool more = it.first(p); more; more = it.advance(p), ++items) {
-        const uint32_t octets = (uint32_t)it.g.octets;
-        float sink = 0.f;
-        if (key < kGroupRows) {
-            const bool there = key < octets * kOctet;
-            const uint64_t row = (uint64_t)it.g.first_octet * kOctet + key;
-            const float *alphas = reinterpret_cast<const float *>(p.at(p.s.alphas));
-            alpha[key] = there ? __ldcg(alphas + row) : 0.f;
-            alpha[64 + key] = there && p.s.kinds == 2u ? __ldcg(alphas + (uint64_t)p.s.octets * kOctet + row) : 0.f;
-            ref[key] = kNoKey;
-            if (there) sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
-        } else if (key < kGroupRows + kGroupOctets) {
-            const uint32_t o = key - kGroupRows;
-            uint64_t m = 0, c = 0;
-            if (o < octets) {
-                const uint32_t token = ((uint32_t)it.g.first_octet + o) / per_token;
-                m = reinterpret_cast<const uint64_t *>(p.a.paths)[token];
-                if (it.g.drafted < (int32_t)kTreeDraft) m &= (1ull << it.g.drafted) - 1ull;
-                if (p.a.cmpPaths) c = reinterpret_cast<const uint64_t *>(p.a.cmpPaths)[token];
+        const uint32_t row0 = half * kRows;                   // first row of the half in the group
+        const bool mine = key < kRows && row0 + key < (uint32_t)it.g.octets * kOctet;          // this thread looks after row `key` of the half
+        {
+            uint64_t *path = reinterpret_cast<uint64_t *>(sm.ptr + kSmPath);
+            float *alpha = sm.floats(kSmAlpha) + row0;
+            if (key < kRows) {
+                const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
+                const float *alphas = reinterpret_cast<const float *>(p.at(p.s.alphas));
+                alpha[key] = mine ? __ldcg(alphas + row) : 0.f;
+                alpha[kGroupRows + key] = mine && p.s.kinds == 2u ? __ldcg(alphas + (uint64_t)p.s.octets * kOctet + row) : 0.f;
+                ref[key] = kNoKey;
+            } else if (key < kRows + kOctets) {
+                const uint32_t o = half * kOctets + key - kRows;
+                uint64_t m = 0, c = 0;
+                if (o < (uint32_t)it.g.octets) {
+                    const uint32_t token = ((uint32_t)it.g.first_octet + o) / per_token;
+                    m = reinterpret_cast<const uint64_t *>(p.a.paths)[token];
+                    if (it.g.drafted < (int32_t)kTreeDraft) m &= (1ull << it.g.drafted) - 1ull;
+                    if (p.a.cmpPaths) c = reinterpret_cast<const uint64_t *>(p.a.cmpPaths)[token];
+                }
+                path[o] = m;
+                path[kGroupOctets + o] = c;
+                reinterpret_cast<int32_t *>(path + 2 * kGroupOctets)[o] = __popcll(m);
             }
-            path[o] = m;
-            cmp_path[o] = c;
-            length[o] = __popcll(m);
         }
-        if (!softmax_sync(sm, phase)) return;
-        const uint32_t present = (1u << octets) - 1u;
-        const int32_t whole_rows = max(it.g.prefix, 0) / 128;
-        float row_sum[2] = {0.f, 0.f};                        // this warp's share of the denominators of rows lane and 32 + lane
+        if (!softmax_sync(sm, half, phase)) return;
+        float row_sum = 0.f;                                  // this warp's share of the denominator of row `lane`
 
         for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
             const bool ori = j < (uint32_t)it.g.ori_tiles;
-            const float *scale = alpha + (ori ? 0 : 64);
             const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
-            // ---- which octets see this key, and how often (a bias of log2 of the count)
+            // ---- which octets see this key, and on ratio-4 layers how often
             uint32_t sees = 0;
-            float bias[LISTED ? 8 : 1];
-            uint4 count = make_uint4(0, 0, 0, 0);
+            uint2 count = make_uint2(0x00010001u, 0x00010001u);
             if (LISTED && !ori) {
                 const uint32_t entry = (j - (uint32_t)it.g.ori_tiles) * kTile + key;
                 const uint64_t at = (uint64_t)it.g.first_octet * p.a.topk + entry;
+                count = make_uint2(0, 0);
                 if (entry < (uint32_t)it.g.cmp_rows && __ldcg(reinterpret_cast<const int32_t *>(p.at(p.s.rows)) + at) >= 0)
-                    count = __ldcg(reinterpret_cast<const uint4 *>(p.at(p.s.counts)) + at);
-            }
-            if (LISTED) {
-                const uint32_t words[4] = {count.x, count.y, count.z, count.w};
-#pragma unroll
-                for (uint32_t o = 0; o < 8; ++o) {
-                    const uint32_t n = (words[o / 2u] >> ((o & 1u) * 16u)) & 0xffffu;
-                    if (n) sees |= 1u << o;
-                    bias[o] = n > 1u ? log2f((float)n) : 0.f;
-                }
-            }
-            if (!LISTED || ori) {
+                    count = __ldcg(reinterpret_cast<const uint2 *>(p.at(p.s.counts)) + 2u * at + half);
+                sees = (count.x & 0xffffu ? 1u : 0u) | (count.x >> 16 ? 2u : 0u) | (count.y & 0xffffu ? 4u : 0u) | (count.y >> 16 ? 8u : 0u);
+            } else {
                 if (!walk_wait<0>(sm, kBarKeyFull + (4u * t) % kRing, ph)) return;      // the page mask comes with segment 0
                 if ((flags[kFlagPages + (t & 3u)] >> warp) & 1u) {
-                    const int32_t row = (ori ? window_page(it.g.prefix, p.a.window) * (int32_t)kTreePage + (int32_t)(j * kTile)
-                                             : (int32_t)((j - (uint32_t)it.g.ori_tiles) * kTile)) + (int32_t)key;
+                    const uint64_t *path = reinterpret_cast<const uint64_t *>(sm.ptr + kSmPath) + half * kOctets;
                     if (ori) {
-                        const int32_t drafted = row - it.g.prefix;
+                        const int32_t *length = reinterpret_cast<const int32_t *>(sm.ptr + kSmPath + 16u * kGroupOctets) + half * kOctets;
+                        const int32_t drafted = window_page(it.g.prefix, p.a.window) * (int32_t)kTreePage + (int32_t)(j * kTile + key) - it.g.prefix;
 #pragma unroll
-                        for (uint32_t o = 0; o < 8; ++o) {
+                        for (uint32_t o = 0; o < kOctets; ++o) {
                             const bool seen = drafted < 0 ? drafted + (int32_t)p.a.window >= length[o]
                                                           : drafted < (int32_t)kTreeDraft && ((path[o] >> drafted) & 1ull);
                             sees |= seen ? 1u << o : 0u;
                         }
-                    } else if (row < whole_rows) {
-                        sees = 0xffu;
-                    } else if (row - whole_rows < (int32_t)kTreeDraft) {
+                    } else {
+                        const int32_t drafted = (int32_t)((j - (uint32_t)it.g.ori_tiles) * kTile + key) - max(it.g.prefix, 0) / 128;
+                        if (drafted < 0) {
+                            sees = 0xfu;
+                        } else if (drafted < (int32_t)kTreeDraft) {
 #pragma unroll
-                        for (uint32_t o = 0; o < 8; ++o) sees |= (uint32_t)((cmp_path[o] >> (row - whole_rows)) & 1ull) << o;
-                    }
-                }
-            }
-            sees &= present;
-            const bool all = __all_sync(0xffffffffu, sees == 0xffu) && !LISTED;
-
-            // ---- logits against the references
-            if (!walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
-            tc_fence_after();
-            float x[kGroupRows];
-            auto logits = [&](bool absolute) {
-#pragma unroll
-                for (uint32_t c = 0; c < 4; ++c) {
-                    uint32_t hi[16], lo[16];
-                    tmem_ld16(tmem_lane + kColScore + buf * kCodeRows + c * 16u, hi);
-                    tmem_ld16(tmem_lane + kColScore + buf * kCodeRows + kGroupRows + c * 16u, lo);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (uint32_t q = 0; q < 4; ++q) {
-                        const float4 a = reinterpret_cast<const float4 *>(scale)[c * 4u + q], m = reinterpret_cast<const float4 *>(ref)[c * 4u + q];
-                        const float as[4] = {a.x, a.y, a.z, a.w}, ms[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            const uint32_t r = q * 4u + i;
-                            float off = absolute ? 0.f : -ms[i];
-                            if (LISTED) off += bias[(c * 16u + r) / kOctet];
-                            x[c * 16u + r] = fmaf((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), as[i], off);
+                            for (uint32_t o = 0; o < kOctets; ++o) sees |= (uint32_t)((path[kGroupOctets + o] >> drafted) & 1ull) << o;
                         }
                     }
                 }
-                if (!all) {
+                const int32_t present = it.g.octets - (int32_t)(half * kOctets);
+                sees &= (1u << max(min(present, (int32_t)kOctets), 0)) - 1u;
+            }
+
+            if (!walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
+            if (t >= 2u && !walk_wait<0>(sm, kBarWeightFree + buf, ph ^ 1u)) return;
+            tc_fence_after();
+            const float *alpha = sm.floats(kSmAlpha) + row0 + (ori ? 0u : kGroupRows);
+            char *weights = sm.ptr + kSmWeight + buf * kSeg + key * 128u;
+            const uint32_t columns = score + buf * kCodeRows;
+            // log2 logits of octet o: integers joined exactly, one conversion, one FMA with the offset
+            auto logits = [&](uint32_t o, bool absolute, float (&x)[8]) {
+                uint32_t hi[8], lo[8];
+                tmem_ld8(columns + o * 8u, hi);
+                tmem_ld8(columns + kGroupRows + o * 8u, lo);
+                float bias = 0.f;
+                if (LISTED) {
+                    const uint32_t n = ((o & 2u ? count.y : count.x) >> ((o & 1u) * 16u)) & 0xffffu;
+                    if (n > 1u) bias = log2f((float)n);
+                }
+                const bool seen = (sees >> o) & 1u;
+                tmem_wait_ld();
 #pragma unroll
-                    for (uint32_t r = 0; r < kGroupRows; ++r) x[r] = (sees >> (r / kOctet)) & 1u ? x[r] : -INFINITY;
+                for (uint32_t q = 0; q < 2; ++q) {
+                    const float4 a = reinterpret_cast<const float4 *>(alpha)[o * 2u + q], m = reinterpret_cast<const float4 *>(ref)[o * 2u + q];
+                    const float as[4] = {a.x, a.y, a.z, a.w}, ms[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const float off = absolute ? bias : LISTED ? bias - ms[i] : -ms[i];
+                        const float v = fmaf((float)((int32_t)hi[4 * q + i] * 254 + (int32_t)lo[4 * q + i]), as[i], off);
+                        x[4 * q + i] = seen ? v : -INFINITY;
+                    }
                 }
             };
-            logits(false);
-            float most = x[0];
+            // The first tile of an item has no references to start from.
+            uint32_t todo = j == it.begin ? 0u : 0xfu, total = 0;
+            bool again = false;
+            for (;;) {
+                uint32_t above = 0;
+#pragma unroll 1
+                for (uint32_t o = 0; o < kOctets; ++o) {
+                    if (!((todo >> o) & 1u)) continue;
+                    float x[8];
+                    logits(o, false, x);
+                    const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                    above |= most > 0.f ? 1u << o : 0u;
+                    uint32_t d[8];
+                    const uint32_t at = lane - o * 8u;
 #pragma unroll
-            for (uint32_t r = 1; r < kGroupRows; ++r) most = fmaxf(most, x[r]);
-            if (most > 0.f) flags[kFlagVote + vote] = 1;
-            if (!softmax_sync(sm, phase)) return;
-            const bool moved = flags[kFlagVote + vote] != 0;
-            vote = vote == 2u ? 0u : vote + 1u;
-            if (key == 0) {
-                // the slot after next was last read before the barrier just passed, and is set behind the next one
-                flags[kFlagVote + (vote == 2u ? 0u : vote + 1u)] = 0;
-                flags[kFlagRescale + buf] = moved;
-            }
-            if (moved) {
-                // exact row maxima: integers in float order, over the lanes by reduction, over the warps by atomicMax
-                logits(true);
-                int32_t high[2] = {INT32_MIN, INT32_MIN};
-#pragma unroll
-                for (uint32_t r = 0; r < kGroupRows; ++r) {
-                    const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x[r])));
-                    if (lane == (r & 31u)) high[r >> 5] = v;
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        d[i] = __float_as_uint(__fmaf_rn(exp2_approx(x[i]), kWeightSteps, 8388736.f));     // 2^23 + 128 + code
+                        const uint32_t sum = __reduce_add_sync(0xffffffffu, d[i]);
+                        if (at == i) total = sum - 32u * kCodeBias;
+                    }
+                    const uint32_t chunk = half * 2u + (o >> 1), place = (o & 1u) * 8u;
+                    *reinterpret_cast<uint2 *>(weights + ((chunk ^ (key & 7u)) << 4) + place) =
+                        make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410),
+                                   __byte_perm(__byte_perm(d[4], d[5], 0x0051), __byte_perm(d[6], d[7], 0x0051), 0x5410));
+                    *reinterpret_cast<uint2 *>(weights + (((4u + chunk) ^ (key & 7u)) << 4) + place) =
+                        make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0040), __byte_perm(d[2], d[3], 0x0040), 0x5410) ^ 0x80808080u,
+                                   __byte_perm(__byte_perm(d[4], d[5], 0x0040), __byte_perm(d[6], d[7], 0x0040), 0x5410) ^ 0x80808080u);
                 }
-                atomicMax(top + lane, high[0]);
-                atomicMax(top + 32 + lane, high[1]);
-                if (!softmax_sync(sm, phase)) return;
-                if (key < kGroupRows) {
+                if (again) break;
+                if (j == it.begin) {
+                    todo = 0xfu;
+                } else {
+                    if (above) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
+                    if (!softmax_sync(sm, half, phase)) return;
+                    todo = flags[vote];
+                    const uint32_t first = kFlagVote + half * 3u;
+                    vote = vote == first + 2u ? first : vote + 1u;
+                    // the word after next was last read before the barrier just passed, and is set behind the next one
+                    if (key == 0) flags[vote == first + 2u ? first : vote + 1u] = 0;
+                }
+                if (key == 0) flags[kFlagRescale + buf * 2u + half] = todo;
+                if (!todo) break;
+                // exact row maxima of the octets concerned: integers in float order
+                int32_t high = INT32_MIN;
+#pragma unroll 1
+                for (uint32_t o = 0; o < kOctets; ++o) {
+                    if (!((todo >> o) & 1u)) continue;
+                    float x[8];
+                    logits(o, true, x);
+                    const uint32_t at = lane - o * 8u;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) {
+                        const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x[i])));
+                        if (at == i) high = v;
+                    }
+                }
+                atomicMax(top + lane, high);
+                if (!softmax_sync(sm, half, phase)) return;
+                float *factors = sm.floats(kSmFactor) + buf * kGroupRows + row0;
+                if (key < kRows) {
                     const float highest = __int_as_float(ordered(top[key])), old = ref[key];
                     float now = old, factor = 1.f;
                     if (highest > old - 1.f) {                // the margin covers the rounding of x; a NaN moves nothing
@@ -843,79 +887,51 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     }
                     top[key] = INT32_MIN;
                     ref[key] = now;
-                    sm.floats(kSmFactor)[buf * kGroupRows + key] = factor;
+                    factors[key] = factor;
                 }
-                if (!softmax_sync(sm, phase)) return;
-                row_sum[0] *= sm.floats(kSmFactor)[buf * kGroupRows + lane];
-                row_sum[1] *= sm.floats(kSmFactor)[buf * kGroupRows + 32u + lane];
-                logits(false);
+                if (!softmax_sync(sm, half, phase)) return;
+                row_sum *= factors[lane];
+                again = true;
             }
             tc_fence_before();
             mbar_arrive(sm.bar(kBarScoreFree + buf));
-
-            // ---- weights as codes
-            if (t >= 2u && !walk_wait<0>(sm, kBarWeightFree + buf, ph ^ 1u)) return;
-            char *weights = sm.ptr + kSmWeight + buf * kSeg + key * 128u;
-            uint32_t total[2] = {0, 0};
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (uint32_t q = 0; q < 4; ++q) {
-                    uint32_t d[4];
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t r = c * 16u + q * 4u + i;
-                        d[i] = __float_as_uint(__fmaf_rn(exp2_approx(x[r]), kWeightSteps, 8388736.f));     // 2^23 + 128 + code
-                        const uint32_t s = __reduce_add_sync(0xffffffffu, d[i]);
-                        if (lane == (r & 31u)) total[r >> 5] = s - 32u * kCodeBias;
-                    }
-                    hi[q] = __byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410);
-                    lo[q] = __byte_perm(__byte_perm(d[0], d[1], 0x0040), __byte_perm(d[2], d[3], 0x0040), 0x5410) ^ 0x80808080u;
-                }
-                *reinterpret_cast<uint4 *>(weights + ((c ^ (key & 7u)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4 *>(weights + (((4u + c) ^ (key & 7u)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
             fence_proxy_async_smem();
             mbar_arrive(sm.bar(kBarWeightReady + buf));
-            row_sum[0] += (float)total[0];
-            row_sum[1] += (float)total[1];
+            row_sum += (float)total;
         }
 
         // ---- denominators, the warps' shares added in warp order
 #pragma unroll 1
         for (uint32_t w = 0; w < 4; ++w) {
-            if (warp == w) {
-                sums[lane] = w ? sums[lane] + row_sum[0] : row_sum[0];
-                sums[32 + lane] = w ? sums[32 + lane] + row_sum[1] : row_sum[1];
-            }
-            if (!softmax_sync(sm, phase)) return;
+            if (warp == w) sums[lane] = w ? sums[lane] + row_sum : row_sum;
+            if (!softmax_sync(sm, half, phase)) return;
         }
         if (!walk_wait<0>(sm, kBarDoneFree, (items & 1u) ^ 1u)) return;
-        if (key < octets * kOctet) {
-            float l = sums[key];
-            if (alpha[key] != alpha[key]) l = alpha[key];     // a query row that is not finite
-            const float m = ref[key];
+        if (mine) {
+            const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
+            const float a = sm.floats(kSmAlpha)[row0 + key], l = a != a ? a : sums[key], m = ref[key];      // NaN: a query row that is not finite
             if (it.whole()) {
+                const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
                 const float sink2 = sink * kLog2e, at = fmaxf(m, sink2), own = exp2_approx(m - at);
                 const float all_sum = l * own + (sink == -INFINITY ? 0.f : kWeightSteps * exp2_approx(sink2 - at));
-                inverse[key] = all_sum == 0.f ? 0.f : own / all_sum;
+                sm.floats(kSmInverse)[row0 + key] = all_sum == 0.f ? 0.f : own / all_sum;
                 if (p.a.lse)
-                    reinterpret_cast<float *>(p.a.lse)[(uint64_t)it.g.first_octet * kOctet + key] =
-                        all_sum == 0.f ? -INFINITY : (at + log2f(all_sum * (1.f / kWeightSteps))) * kLn2;
+                    reinterpret_cast<float *>(p.a.lse)[row] = all_sum == 0.f ? -INFINITY : (at + log2f(all_sum * (1.f / kWeightSteps))) * kLn2;
             } else {
-                float *mine = reinterpret_cast<float *>(p.at(p.s.partials)) + (uint64_t)it.partial() * kPartial + kGroupRows * kDim;
-                mine[key] = l;
-                mine[kGroupRows + key] = m;
+                float *partial = reinterpret_cast<float *>(p.at(p.s.partials)) + (uint64_t)it.partial() * kPartial + kGroupRows * kDim + row0;
+                partial[key] = l;
+                partial[kGroupRows + key] = m;
             }
         }
         mbar_arrive(sm.bar(kBarDone));
     }
 }
 
-// ------------------------------------------------------------------ walk: accumulate (warps 4-11)
+// ------------------------------------------------------------------ walk: accumulate (warps 8-15)
 // Thread = channel of each 128-channel block, rows 32 h .. 32 h + 31: 128 running sums in registers.  The
-// integers of a block are read, joined, scaled and added while the tensor core fills the other block.
+// integers of a block are read, joined and added while the tensor core fills the other block.  Sums are in
+// units of the current kind's channel scale: they change units where an item goes from one kind to the
+// other, and are scaled when they are stored.
 __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
 {
     const uint32_t index = threadIdx.x - kWarpAccumulate * 32u, h = index >> 7, channel = index & 127u, warp = channel >> 5;
@@ -931,7 +947,16 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
         for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
             const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
             if (!walk_wait<1>(sm, kBarWeightReady + buf, ph)) return;
-            if (sm.flags()[kFlagRescale + buf]) {
+            if (j == (uint32_t)it.g.ori_tiles && j != it.begin) {
+#pragma unroll
+                for (int block = 0; block < 4; ++block) {
+                    const float units = __ldg(reinterpret_cast<const float *>(p.a.oriScale) + block * 128 + channel) /
+                                        __ldg(reinterpret_cast<const float *>(p.a.cmpScale) + block * 128 + channel);
+#pragma unroll
+                    for (int r = 0; r < 32; ++r) acc[block][r] *= units;
+                }
+            }
+            if (sm.flags()[kFlagRescale + buf * 2u + h]) {
                 const float4 *factor = reinterpret_cast<const float4 *>(sm.ptr + kSmFactor) + buf * 16u + h * 8u;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
@@ -943,10 +968,8 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     }
                 }
             }
-            const float *scale = reinterpret_cast<const float *>(j < (uint32_t)it.g.ori_tiles ? p.a.oriScale : p.a.cmpScale) + channel;
 #pragma unroll
             for (uint32_t block = 0; block < 4; ++block) {
-                const float s = __ldg(scale + block * 128u);
                 const uint32_t half = block & 1u;
                 if (!walk_wait<1>(sm, kBarOutFull + half, (block >> 1) & 1u)) return;
                 tc_fence_after();
@@ -958,7 +981,7 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     tmem_wait_ld();
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i)
-                        acc[block][c * 8u + i] = fmaf((float)((int32_t)hi[i] * 256 + (int32_t)lo[i]), s, acc[block][c * 8u + i]);
+                        acc[block][c * 8u + i] += (float)((int32_t)hi[i] * 256 + (int32_t)lo[i]);
                 }
                 tc_fence_before();
                 mbar_arrive(sm.bar(kBarOutFree + half));
@@ -966,6 +989,13 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
         }
         if (!walk_wait<1>(sm, kBarDone, items & 1u)) return;
         const uint32_t rows = (uint32_t)it.g.octets * kOctet;
+        const float *scale = reinterpret_cast<const float *>(it.end <= (uint32_t)it.g.ori_tiles ? p.a.oriScale : p.a.cmpScale) + channel;
+#pragma unroll
+        for (uint32_t block = 0; block < 4; ++block) {
+            const float f = __ldg(scale + block * 128u);
+#pragma unroll
+            for (uint32_t r = 0; r < 32; ++r) acc[block][r] *= f;
+        }
         if (it.whole()) {
             const float *inverse = sm.floats(kSmInverse) + h * 32u;
             __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.a.out) + ((uint64_t)it.g.first_octet * kOctet + h * 32u) * kDim + channel;
@@ -1005,14 +1035,15 @@ __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid
         mbar_init(sm.bar(kBarQueryFull), 1);
         mbar_init(sm.bar(kBarQueryEmpty), 1);
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(sm.bar(kBarScoreFull + i), 1); mbar_init(sm.bar(kBarScoreFree + i), 128);
-            mbar_init(sm.bar(kBarWeightReady + i), 128); mbar_init(sm.bar(kBarWeightFree + i), 1);
+            mbar_init(sm.bar(kBarScoreFull + i), 1); mbar_init(sm.bar(kBarScoreFree + i), 256);
+            mbar_init(sm.bar(kBarWeightReady + i), 256); mbar_init(sm.bar(kBarWeightFree + i), 1);
             mbar_init(sm.bar(kBarOutFull + i), 1); mbar_init(sm.bar(kBarOutFree + i), 256);
         }
         mbar_init(sm.bar(kBarSync), 128);
-        mbar_init(sm.bar(kBarDone), 128);
+        mbar_init(sm.bar(kBarSync + 1), 128);
+        mbar_init(sm.bar(kBarDone), 256);
         mbar_init(sm.bar(kBarDoneFree), 256);
-        for (uint32_t i = 0; i < 12; ++i) if (i != kFlagTmem) flags[i] = 0;
+        for (uint32_t i = 0; i < 16; ++i) if (i != kFlagTmem) flags[i] = 0;
         fence_mbar_init();
     }
     if (warp == kWarpIssue) {
@@ -1027,6 +1058,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid
     grid_dependency_wait();
 
     if (warp < kWarpAccumulate) {
+        registers_release<kRegsSoftmax>();
         softmax<LISTED>(p, sm, tmem);
     } else if (warp < kWarpIssue) {
         registers_acquire<kRegsAccumulate>();
@@ -1192,7 +1224,8 @@ int tree_launch_all(const TreeAttentionArgs &a, cudaStream_t stream, int sms)
         !tree_map(&row_map, a.cmp, a.cmpStride, a.cmpPages, listed && gather ? 0u : 1u))
         return SHAREDKV_EINVAL;
     static std::atomic<uint64_t> walk_pages{0}, walk_rows{0}, unions{0};
-    cudaError_t e = tree_launch(tree_encode_kernel, dim3(p.s.octets), kEncodeThreads, 0u, stream, p);
+    const uint32_t encode_blocks = p.s.octets < 4u * (uint32_t)sms ? p.s.octets : 4u * (uint32_t)sms;
+    cudaError_t e = tree_launch(tree_encode_kernel, dim3(encode_blocks), kEncodeThreads, 0u, stream, p);
     if (e == cudaSuccess && listed) {
         e = tree_opt_in(tree_union_kernel, kUnionSmem, unions);
         if (e == cudaSuccess) e = tree_launch(tree_union_kernel, dim3(p.s.slots), kUnionThreads, kUnionSmem, stream, p);
