@@ -20,9 +20,9 @@
 // per row that stays at or above every logit so far; weights 2^x <= 1 become codes c = rint(32639 * 2^x) = 256 c_hi + c_lo
 // (15 bits, c_lo signed), so O = 256 O_hi + O_lo is again one exact integer per tile, summed over tiles in
 // FP32 registers; the denominator is the sum of the same codes.  The reference moves only when some
-// logit exceeds it, and then to two powers of two above that logit (kHeadroom): the exact row maximum, a
-// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  The 2 bits this
-// takes from the codes leave steps of 2^-13 of the largest weight, below a BF16 result's 2^-8.
+// logit exceeds it, and then to three powers of two above that logit (kHeadroom): the exact row maximum, a
+// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  The 3 bits this
+// takes from the codes leave steps of 2^-12 of the largest weight, below a BF16 result's 2^-8.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -48,15 +48,15 @@ constexpr uint32_t kSeg = kTile * 128;                       // one 128-channel 
 constexpr uint32_t kRing = 8;                                // segments in flight: two tiles
 constexpr uint32_t kWalkThreads = 640;
 constexpr uint32_t kEncodeThreads = 256, kUnionThreads = 1024, kMergeThreads = 256;
-constexpr uint32_t kWarpAccumulate = 8, kWarpIssue = 16, kWarpProduce = 17, kProducers = 3;
+constexpr uint32_t kWarpAccumulate = 8, kWarpIssue = 16, kWarpProduce = 18, kProducers = 2;
 // Registers: launched with 96 per thread; accumulate (two warps of every SM partition) grows to hold
 // 128 running sums a thread, the others shrink.
-constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 56, kRegsAccumulate = 168, kRegsIssue = 32;
+constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 72, kRegsAccumulate = 152, kRegsIssue = 32;
 static_assert(2 * kRegsSoftmax + 2 * kRegsAccumulate + kRegsIssue <= 5 * kRegsLaunch, "register shares exceed the launch allocation");
 constexpr float kWeightSteps = 32639.f;                      // 127 * 256 + 127: the largest weight code
 constexpr uint32_t kCodeBias = 0x4b000080u;                  // bits of 2^23 + 128
 constexpr float kNoKey = -1e30f;                             // reference of a row that has met no key
-constexpr float kHeadroom = 2.f;
+constexpr float kHeadroom = 3.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows a union bitmap covers at a time (32 KB)
 constexpr uint32_t kTreeWaitMillions = 4000;                 // cycles, ~2 s: a wait that long is a failure
@@ -68,7 +68,7 @@ constexpr uint32_t kSmKey = 0;
 constexpr uint32_t kSmQuery = kSmKey + kRing * kSeg;         // 64 KB: four segments of 128 code rows
 constexpr uint32_t kSmWeight = kSmQuery + 4 * kSeg;          // two tiles of weight codes, 128 keys x 128 bytes
 constexpr uint32_t kSmAlpha = kSmWeight + 2 * kSeg;          // FP32 [2 kinds][64]
-constexpr uint32_t kSmRef = kSmAlpha + 512;                  // FP32 [64]
+constexpr uint32_t kSmRef = kSmAlpha + 512;                  // FP32 [64], negated
 constexpr uint32_t kSmTop = kSmRef + 256;                    // INT32 [64] row maxima, as ordered integers
 constexpr uint32_t kSmFactor = kSmTop + 256;                 // FP32 [2][64] rescale factors of a tile
 constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [64] denominators
@@ -76,9 +76,9 @@ constexpr uint32_t kSmInverse = kSmSum + 256;                // FP32 [64]
 constexpr uint32_t kSmPath = kSmInverse + 256;               // UINT64 [8] paths, UINT64 [8] compressed paths, INT32 [8] path lengths
 constexpr uint32_t kSmFlags = kSmPath + 160;                 // rescale [2 tiles][2 halves], vote [2 halves][3], page masks [4], tmem base, abort
 constexpr uint32_t kSmBars = kSmFlags + 64;
-constexpr uint32_t kBarKeyFull = 0, kBarKeyEmpty = 8, kBarQueryFull = 16, kBarQueryEmpty = 17, kBarScoreFull = 18, kBarScoreFree = 20,
-                   kBarWeightReady = 22, kBarWeightFree = 24, kBarOutFull = 26, kBarOutFree = 28, kBarSync = 30, kBarDone = 32,
-                   kBarDoneFree = 33, kTreeBars = 34;
+constexpr uint32_t kBarKeyFull = 0, kBarKeyEmpty = 8 /* per two segments */, kBarQueryFull = 12, kBarQueryEmpty = 13, kBarScoreFull = 14,
+                   kBarScoreFree = 16, kBarWeightReady = 18, kBarOutFull = 20, kBarOutFree = 22, kBarSync = 24, kBarDone = 26,
+                   kBarDoneFree = 27, kTreeBars = 28;
 constexpr uint32_t kWalkSmem = kSmBars + 8 * kTreeBars;
 static_assert(kWalkSmem <= 232448, "dynamic shared memory limit of sm_100");
 static_assert(kSmPath % 8 == 0 && kSmBars % 8 == 0, "64-bit words");
@@ -129,6 +129,34 @@ struct Tree {
     __device__ __forceinline__ uint32_t *head() const { return reinterpret_cast<uint32_t *>(a.workspace); }
 };
 
+// Two FP32 values to a register pair, for the packed FMA and add.
+__device__ __forceinline__ uint64_t pack2(float a, float b)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float low2(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high2(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+
 // Descriptor slot of the j-th group of request b.  floor(x + y) + 1 >= floor(x) + ceil(y), so requests
 // do not run into each other and the slots are in request order; the ones between stay empty.
 __device__ __forceinline__ uint32_t slot_of(uint32_t octets_before, uint32_t request, uint32_t j) { return octets_before / kGroupOctets + request + j; }
@@ -155,7 +183,7 @@ __device__ __forceinline__ int32_t window_page(int32_t prefix, uint32_t window)
 // ------------------------------------------------------------------ work split
 // Runs in the last block of the kernel in front of the walk.  The tiles of all groups, each group with
 // kGroupCost units in front, are cut into p.grid ranges of equal cost; a cut that would leave a piece of fewer than
-// kMinPiece tiles moves to the group's edge.  Cut i is (slot, tile): block i walks from cut i to cut i + 1.
+// kMinPiece tiles (half a range where that is less: with little work, tiles run side by side) moves to the group's edge.  Cut i is (slot, tile): block i walks from cut i to cut i + 1.
 __device__ void cut_tiles(const Tree &p)
 {
     __shared__ uint32_t sums[33];
@@ -195,6 +223,7 @@ __device__ void cut_tiles(const Tree &p)
     if (threadIdx.x == 0) starts[p.s.slots] = total;
     __syncthreads();
     const uint32_t quota = total ? (total + p.grid - 1u) / p.grid : 1u;
+    const uint32_t shortest = max(1u, min(quota / 2u, kMinPiece));
     uint2 *cuts = reinterpret_cast<uint2 *>(p.at(p.s.cuts));
     for (uint32_t i = threadIdx.x; i <= p.grid; i += blockDim.x) {
         const uint32_t position = i * quota;
@@ -206,7 +235,7 @@ __device__ void cut_tiles(const Tree &p)
         }
         const uint32_t inside = position - starts[lo], tiles = starts[lo + 1u] - starts[lo] - kGroupCost;
         const uint32_t tile = inside > kGroupCost ? inside - kGroupCost : 0u;
-        cuts[i] = tile < kMinPiece ? make_uint2(lo, 0) : tiles - tile < kMinPiece ? make_uint2(lo + 1u, 0) : make_uint2(lo, tile);
+        cuts[i] = tile < shortest ? make_uint2(lo, 0) : tiles - tile < shortest ? make_uint2(lo + 1u, 0) : make_uint2(lo, tile);
     }
 }
 
@@ -227,32 +256,37 @@ __device__ bool last_block(const Tree &p, uint32_t blocks)
 // A block takes octets in turn, a warp per head: lane l owns channels 16 l .. 16 l + 15, one 16-byte chunk of a code
 // row.  Codes go out as the walk's B operand wants them: [kind][segment][plane][octet] blocks of 8 rows x
 // 128 bytes, swizzled, so that a group's rows of a plane are one contiguous copy.
-__device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_t octet, uint32_t row, const float (&q)[16], const float *sm_scale)
+__device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_t octet, uint32_t row, const uint64_t (&q)[8], const float *sm_scale)
 {
     const uint32_t lane = threadIdx.x & 31u;
-    const float4 *scale = reinterpret_cast<const float4 *>(sm_scale + kind * kDim) + lane;      // [4][32 lanes]: no bank conflicts
-    float f[16];
-    uint32_t top = 0;                                         // largest |f| as an integer: a NaN or an infinity wins
+    const ulonglong2 *scale = reinterpret_cast<const ulonglong2 *>(sm_scale + kind * kDim) + lane;      // [4][32 lanes]: no bank conflicts
+    uint64_t f[8];
+    float top = 0.f;                                          // largest |f|; a NaN stays one
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float4 v = scale[i * 32];
-        f[4 * i] = q[4 * i] * v.x; f[4 * i + 1] = q[4 * i + 1] * v.y; f[4 * i + 2] = q[4 * i + 2] * v.z; f[4 * i + 3] = q[4 * i + 3] * v.w;
+        const ulonglong2 v = scale[i * 32];
+        f[2 * i] = mul2(q[2 * i], v.x);
+        f[2 * i + 1] = mul2(q[2 * i + 1], v.y);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    const bool finite = top < 0x7f800000u;
-    const float alpha = fmaxf(__uint_as_float(top) * (float)(1.0 / 127), 1e-30f), rcp = __frcp_rn(alpha);
+    for (int i = 0; i < 8; ++i) {
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(low2(f[i]))));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(high2(f[i]))));
+    }
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));        // as integers a NaN is above all
+    const bool finite = bits < 0x7f800000u;
+    const float alpha = fmaxf(__uint_as_float(bits) * (float)(1.0 / 127), 1e-30f), rcp = __frcp_rn(alpha);
+    // adding 1.5 * 2^23 leaves the nearest integer in the low bits of the sum
+    const uint64_t rcp2 = pack2(rcp, rcp), magic = pack2(12582912.f, 12582912.f), minus = pack2(-1.f, -1.f), low = pack2(254.f, 254.f);
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        // adding 1.5 * 2^23 leaves the nearest integer in the low bits of the sum
         uint32_t ch[4], cl[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float n = f[4 * w + e] * rcp, shifted = __fadd_rn(n, 12582912.f), rest = __fsub_rn(n, __fsub_rn(shifted, 12582912.f));
-            ch[e] = __float_as_uint(shifted);
-            cl[e] = __float_as_uint(__fadd_rn(__fmul_rn(rest, 254.f), 12582912.f));
+        for (int e = 0; e < 2; ++e) {
+            const uint64_t v = f[2 * w + e], h = fma2(v, rcp2, magic), l = fma2(fma2(v, rcp2, fma2(h, minus, magic)), low, magic);
+            ch[2 * e] = (uint32_t)h; ch[2 * e + 1] = (uint32_t)(h >> 32);
+            cl[2 * e] = (uint32_t)l; cl[2 * e + 1] = (uint32_t)(l >> 32);
         }
         hi[w] = __byte_perm(__byte_perm(ch[0], ch[1], 0x0040), __byte_perm(ch[2], ch[3], 0x0040), 0x5410);
         lo[w] = __byte_perm(__byte_perm(cl[0], cl[1], 0x0040), __byte_perm(cl[2], cl[3], 0x0040), 0x5410);
@@ -319,6 +353,11 @@ __global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __gri
     }
     for (uint32_t octet = blockIdx.x; octet < p.s.octets; octet += gridDim.x) {
         const uint32_t token = octet / per_token;
+        uint64_t q[8];
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = pack2(__uint_as_float(words[i] << 16), __uint_as_float(words[i] & 0xffff0000u));
+        if (octet + gridDim.x < p.s.octets) fetch(octet + gridDim.x, raw);             // the next octet's rows are on their way
         if (token >= live_tokens || (int32_t)token < cu[0]) {
             const uint64_t at = ((uint64_t)octet * kOctet + row) * kDim;
             uint4 *out = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.a.out) + at) + lane * 2u;
@@ -326,11 +365,6 @@ __global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __gri
             if (p.a.lse && lane == 0) reinterpret_cast<float *>(p.a.lse)[(uint64_t)octet * kOctet + row] = 0.f;
             continue;
         }
-        if (octet != blockIdx.x) fetch(octet, raw);
-        float q[16];
-        const uint32_t *words = reinterpret_cast<const uint32_t *>(raw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { q[2 * i] = __uint_as_float(words[i] << 16); q[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u); }
 #pragma unroll 1
         for (uint32_t kind = 0; kind < p.s.kinds; ++kind) encode_row(p, kind, octet, row, q, sm_scale);
     }
@@ -473,11 +507,22 @@ __device__ __forceinline__ bool walk_wait(const WalkShared &sm, uint32_t bar_ind
     return walk_wait_slow<ROLE>(bar, parity, sm.flags());
 }
 
-// The block's items in order: groups, the first and last possibly in part.  The next descriptor is
-// read while the current item is worked on.
+// The block's items in order: groups, the first and last possibly in part.  AHEAD: the next descriptor is read
+// while the current item is worked on (eight registers that not every role has).
+template <bool AHEAD>
 struct Items {
     uint32_t slot, last_slot, last_tile, begin, end;
     Group g, next;
+    __device__ __forceinline__ void step(const Tree &p)
+    {
+        ++slot;
+        if (AHEAD) {
+            g = next;
+            next = load(p, slot + 1u);
+        } else {
+            g = load(p, slot);
+        }
+    }
     __device__ __forceinline__ Group load(const Tree &p, uint32_t at) const
     {
         Group v = {};
@@ -496,9 +541,7 @@ struct Items {
             begin = from;
             if (slot >= p.s.slots || slot > last_slot) return false;
             if (begin < end) return true;
-            g = next;
-            ++slot;
-            next = load(p, slot + 1u);
+            step(p);
         }
     }
     __device__ __forceinline__ bool first(const Tree &p)
@@ -507,14 +550,12 @@ struct Items {
         const uint2 a = __ldcg(cuts), b = __ldcg(cuts + 1);
         slot = a.x; last_slot = b.x; last_tile = b.y;
         g = load(p, slot);
-        next = load(p, slot + 1u);
+        if (AHEAD) next = load(p, slot + 1u);
         return open(p, a.y);
     }
     __device__ __forceinline__ bool advance(const Tree &p)
     {
-        g = next;
-        ++slot;
-        next = load(p, slot + 1u);
+        step(p);
         return open(p, 0u);
     }
     __device__ __forceinline__ bool whole() const { return begin == 0 && end == (uint32_t)g.tiles; }
@@ -524,130 +565,111 @@ struct Items {
 };
 
 // ------------------------------------------------------------------ walk: producers
-// Three warps take the segments of the tiles in turn: 128 channels of 128 keys, 16 KB.  Pages come as
+// Two warps take the segments of the tiles in turn: 128 channels of 128 keys, 16 KB.  Pages come as
 // whole boxes of 32 rows x 128 bytes; the listed rows of a ratio-4 layer by gathers of four rows, or
-// row by row when the page stride is no multiple of a row.
+// row by row when the page stride is no multiple of a row.  Lanes look up pages and rows.  Boxes go out from
+// one elected lane with operands that are the same in the whole warp (51 cycles a box with two warps, 78 when
+// four lanes issue their own); 32 gathers are issued by their lanes.
 template <bool LISTED>
 __device__ void produce(const Tree &p, const WalkShared &sm, uint32_t mine, const CUtensorMap *ori_map, const CUtensorMap *cmp_map,
                         const CUtensorMap *row_map, bool gather)
 {
     const uint32_t lane = threadIdx.x & 31u;
-    Items it;
-    uint32_t tile = 0, turn = 0;                              // tiles of the block so far; segment number modulo kProducers
+    const bool leader = elect_one();
+    Items<true> it;
+    uint32_t tile = 0;                                        // tiles of the block so far: this warp takes segments mine and mine + 2
     for (bool more = it.first(p); more; more = it.advance(p)) {
         for (uint32_t j = it.begin; j < it.end; ++j, ++tile) {
             const bool ori = j < (uint32_t)it.g.ori_tiles;
+            int32_t at[4] = {-1, -1, -1, -1};
+            uint32_t there, bytes;
             if (LISTED && !ori) {
-                // lane l fetches rows 4 l .. 4 l + 3 of the tile
+                // lane l looks up rows 4 l .. 4 l + 3 of the tile
                 const uint32_t row = (j - (uint32_t)it.g.ori_tiles) * kTile + 4u * lane;
                 const int32_t *list = reinterpret_cast<const int32_t *>(p.at(p.s.rows)) + (uint64_t)it.g.first_octet * p.a.topk;
-                int32_t at[4];
-                uint32_t there = 0;
+                uint32_t found = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     at[i] = row + i < (uint32_t)it.g.cmp_rows ? __ldcg(list + row + i) : -1;
-                    there += at[i] >= 0;
+                    found += at[i] >= 0;
                 }
-                const uint32_t per_page = (uint32_t)(p.a.cmpStride / kDim);
-                const uint32_t bytes = gather ? 512u * __popc(__ballot_sync(0xffffffffu, there != 0))
-                                              : 128u * __reduce_add_sync(0xffffffffu, there);
-#pragma unroll 1
-                for (uint32_t seg = 0; seg < 4; ++seg) {
-                    const bool take = turn == mine;
-                    turn = turn + 1u == kProducers ? 0u : turn + 1u;
-                    if (!take) continue;
-                    const uint32_t slot = (4u * tile + seg) % kRing;
-                    if (!walk_wait<2>(sm, kBarKeyEmpty + slot, ((tile >> 1) & 1u) ^ 1u)) return;
-                    if (lane == 0) mbar_arrive_expect_tx(sm.bar(kBarKeyFull + slot), bytes);
-                    __syncwarp();
-                    const uint32_t dst = sm.base + kSmKey + slot * kSeg + lane * 512u;
-                    if (gather) {
-                        int32_t r[4];
+                there = __ballot_sync(0xffffffffu, found != 0);
+                bytes = gather ? 512u * __popc(there) : 128u * __reduce_add_sync(0xffffffffu, found);
+                if (gather) {
+                    const uint32_t per_page = (uint32_t)(p.a.cmpStride / kDim);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)           // a missing row reads as zeros from beyond the map
-                            r[i] = at[i] < 0 ? 0x7ffffff0 : (int32_t)((uint32_t)at[i] / kTreePage * per_page + (uint32_t)at[i] % kTreePage);
-                        if (there) tma_gather4(dst, row_map, (int32_t)(seg * 128u), r[0], r[1], r[2], r[3], sm.bar(kBarKeyFull + slot));
+                    for (int i = 0; i < 4; ++i)               // a missing row reads as zeros from beyond the map
+                        at[i] = at[i] < 0 ? 0x7ffffff0 : (int32_t)((uint32_t)at[i] / kTreePage * per_page + (uint32_t)at[i] % kTreePage);
+                }
+            } else {
+                // lane l < 4 looks up the tile's l-th page
+                const int32_t *table = reinterpret_cast<const int32_t *>(ori ? p.a.oriTable : p.a.cmpTable);
+                const uint32_t width = ori ? p.a.oriTableWidth : p.a.cmpTableWidth;
+                const uint32_t index = (ori ? (uint32_t)window_page(it.g.prefix, p.a.window) + j * 4u : (j - (uint32_t)it.g.ori_tiles) * 4u) + lane;
+                if (lane < 4 && index < width) at[0] = table[(uint64_t)it.g.request * width + index];
+                there = __ballot_sync(0xffffffffu, (uint32_t)at[0] < (ori ? p.a.oriPages : p.a.cmpPages)) & 15u;
+                bytes = 4096u * __popc(there);
+            }
+#pragma unroll 1
+            for (uint32_t seg = mine; seg < 4u; seg += kProducers) {
+                const uint32_t slot = (4u * tile + seg) % kRing;
+                if (!walk_wait<2>(sm, kBarKeyEmpty + slot / 2u, ((tile >> 1) & 1u) ^ 1u)) return;
+                __syncwarp();
+                const uint32_t full = sm.bar(kBarKeyFull + slot), dst = sm.base + kSmKey + slot * kSeg;
+                if (leader) {
+                    if (seg == 0) sm.flags()[kFlagPages + (tile & 3u)] = there;
+                    mbar_arrive_expect_tx(full, bytes);
+                }
+                if (LISTED && !ori) {
+__syncwarp();
+                    if (gather) {
+                        if ((there >> lane) & 1u) tma_gather4(dst + lane * 512u, row_map, (int32_t)(seg * 128u), at[0], at[1], at[2], at[3], full);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (at[i] >= 0)
-                                tma_page_rows(dst + i * 128u, row_map, (int32_t)(seg * 128u), at[i] % (int32_t)kTreePage, at[i] / (int32_t)kTreePage,
-                                              sm.bar(kBarKeyFull + slot));
+                                tma_page_rows(dst + lane * 512u + i * 128u, row_map, (int32_t)(seg * 128u), at[i] % (int32_t)kTreePage,
+                                              at[i] / (int32_t)kTreePage, full);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const int32_t page = __shfl_sync(0xffffffffu, at[0], i);
+                        if (leader && ((there >> i) & 1u)) tma_page_rows(dst + i * 4096u, ori ? ori_map : cmp_map, (int32_t)(seg * 128u), 0, page, full);
                     }
                 }
-            } else {
-                // lane l < 4 fetches the tile's l-th page
-                const int32_t *table = reinterpret_cast<const int32_t *>(ori ? p.a.oriTable : p.a.cmpTable);
-                const uint32_t width = ori ? p.a.oriTableWidth : p.a.cmpTableWidth;
-                const uint32_t index = (ori ? (uint32_t)window_page(it.g.prefix, p.a.window) + j * 4u : (j - (uint32_t)it.g.ori_tiles) * 4u) + lane;
-                int32_t page = -1;
-                if (lane < 4 && index < width) page = table[(uint64_t)it.g.request * width + index];
-                const bool there = (uint32_t)page < (ori ? p.a.oriPages : p.a.cmpPages);
-                const uint32_t mask = __ballot_sync(0xffffffffu, there) & 15u;
-#pragma unroll 1
-                for (uint32_t seg = 0; seg < 4; ++seg) {
-                    const bool take = turn == mine;
-                    turn = turn + 1u == kProducers ? 0u : turn + 1u;
-                    if (!take) continue;
-                    const uint32_t slot = (4u * tile + seg) % kRing;
-                    if (!walk_wait<2>(sm, kBarKeyEmpty + slot, ((tile >> 1) & 1u) ^ 1u)) return;
-                    if (lane == 0) {
-                        if (seg == 0) sm.flags()[kFlagPages + (tile & 3u)] = mask;
-                        mbar_arrive_expect_tx(sm.bar(kBarKeyFull + slot), 4096u * __popc(mask));
-                    }
-                    __syncwarp();
-                    if (lane < 4 && there)
-                        tma_page_rows(sm.base + kSmKey + slot * kSeg + lane * 4096u, ori ? ori_map : cmp_map, (int32_t)(seg * 128u), 0, page,
-                                      sm.bar(kBarKeyFull + slot));
-                }
+                __syncwarp();
             }
         }
     }
 }
 
 // ------------------------------------------------------------------ walk: issue
-// One warp issues both products (its elected lane; the warp stays converged).  The scores of tile t + 1
-// go out before the output product of tile t, which waits for the weights, so the tensor core works while the
-// softmax does.  The query codes of an item's kind are one resident set of 64 KB; they are replaced
-// once the last score product that reads them has completed.
-__device__ void issue(const Tree &p, const WalkShared &sm, uint32_t tmem)
+// Two warps issue one product each (an elected lane; the warp stays converged): a warp's serial work
+// between two products, waits and commits, takes as long as the products, and would hold up the other kind.  What
+// loops and addresses depend on is broadcast, so that the compiler sees one value for the warp and keeps
+// the operand descriptors in uniform registers.
+__device__ __forceinline__ uint32_t same(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// S[128 keys, 128 code rows] = K . Q^T.  The query codes of an item's kind are one resident set of 64 KB; they
+// are replaced once the last product that reads them has completed.
+__device__ void issue_scores(const Tree &p, const WalkShared &sm, uint32_t tmem)
 {
-    constexpr uint32_t kScore = idesc_i8(128, kCodeRows, 0, 0), kOut = idesc_i8(128, kCodeRows, 1, 1);
+    constexpr uint32_t kScore = idesc_i8(128, kCodeRows, 0, 0);
     const bool leader = elect_one();
-    auto output_product = [&](uint32_t t) {
-        const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
-        if (!walk_wait<3>(sm, kBarWeightReady + buf, ph)) return false;
-        const uint64_t b0 = smem_desc(sm.base + kSmWeight + buf * kSeg, kSeg, 1024u, kSwizzle128);
-#pragma unroll 1
-        for (uint32_t block = 0; block < 4; ++block) {
-            const uint32_t half = block & 1u, use = 2u * t + (block >> 1), slot = (4u * t + block) % kRing;
-            if (!walk_wait<3>(sm, kBarOutFree + half, (use & 1u) ^ 1u)) return false;
-            tc_fence_after();
-            const uint64_t a0 = smem_desc(sm.base + kSmKey + slot * kSeg, kSeg, 1024u, kSwizzle128);
-            if (leader) {
-#pragma unroll
-                for (uint32_t k = 0; k < 4; ++k)
-                    mma_i8(tmem + kColOut + half * kCodeRows, a0 + ((k * 4096u) >> 4), b0 + ((k * 4096u) >> 4), kOut, k);
-                mma_commit(sm.bar(kBarOutFull + half));
-                mma_commit(sm.bar(kBarKeyEmpty + slot));      // the segment's last reader
-                if (block == 3) mma_commit(sm.bar(kBarWeightFree + buf));
-            }
-            __syncwarp();
-        }
-        return true;
-    };
-    Items it;
+    const uint64_t keys = smem_desc(sm.base + kSmKey, 16u, 1024u, kSwizzle128), query = smem_desc(sm.base + kSmQuery, 16u, 1024u, kSwizzle128);
+    Items<true> it;
     uint32_t t = 0, sets = 0;
-    for (bool more = it.first(p); more; more = it.advance(p)) {
-        for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
-            const uint32_t ori_tiles = (uint32_t)it.g.ori_tiles, kind = j < ori_tiles ? 0u : 1u;
-            if (j == it.begin || j == ori_tiles) {
+    for (bool more = same(it.first(p)); more; more = same(it.advance(p))) {
+        const uint32_t begin = same(it.begin), end = same(it.end), ori_tiles = same((uint32_t)it.g.ori_tiles);
+        const uint32_t bytes = 1024u * same((uint32_t)it.g.octets), first_octet = same((uint32_t)it.g.first_octet);
+        for (uint32_t j = begin; j < end; ++j, ++t) {
+            if (j == begin || j == ori_tiles) {
                 if (sets && !walk_wait<3>(sm, kBarQueryEmpty, (sets - 1u) & 1u)) return;
-                const uint32_t bytes = 1024u * (uint32_t)it.g.octets;
                 if (leader) {
                     mbar_arrive_expect_tx(sm.bar(kBarQueryFull), 8u * bytes);
                     const uint64_t plane = 1024ull * p.s.octets;
-                    const char *src = p.at(p.s.codes) + kind * 8ull * plane + 1024ull * (uint32_t)it.g.first_octet;
+                    const char *src = p.at(p.s.codes) + (j < ori_tiles ? 0ull : 8ull * plane) + 1024ull * first_octet;
 #pragma unroll 1
                     for (uint32_t i = 0; i < 8; ++i)
                         bulk_load(sm.base + kSmQuery + (i >> 1) * kSeg + (i & 1u) * (kSeg / 2u), src + i * plane, bytes, sm.bar(kBarQueryFull));
@@ -659,28 +681,52 @@ __device__ void issue(const Tree &p, const WalkShared &sm, uint32_t tmem)
             const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
             if (!walk_wait<3>(sm, kBarScoreFree + buf, ph ^ 1u)) return;
             tc_fence_after();
-#pragma unroll 1
-            for (uint32_t seg = 0; seg < 4; ++seg) {
-                const uint32_t slot = (4u * t + seg) % kRing;
-                if (!walk_wait<3>(sm, kBarKeyFull + slot, ph)) return;
-                const uint64_t a0 = smem_desc(sm.base + kSmKey + slot * kSeg, 16u, 1024u, kSwizzle128);
-                const uint64_t b0 = smem_desc(sm.base + kSmQuery + seg * kSeg, 16u, 1024u, kSwizzle128);
-                if (leader) {
+            const uint64_t a0 = keys + buf * ((4u * kSeg) >> 4);
+            const uint32_t d = tmem + kColScore + buf * kCodeRows;
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)
-                        mma_i8(tmem + kColScore + buf * kCodeRows, a0 + ((k * 32u) >> 4), b0 + ((k * 32u) >> 4), kScore, seg | k);
-                }
-                __syncwarp();
+            for (uint32_t seg = 0; seg < 4; ++seg) {
+                if (!walk_wait<3>(sm, kBarKeyFull + buf * 4u + seg, ph)) return;
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k)
+                    if (leader) mma_i8(d, a0 + ((seg * kSeg + k * 32u) >> 4), query + ((seg * kSeg + k * 32u) >> 4), kScore, seg | k);
             }
             if (leader) {
                 mma_commit(sm.bar(kBarScoreFull + buf));
-                if (j + 1u == it.end || j + 1u == ori_tiles) mma_commit(sm.bar(kBarQueryEmpty));
+                if (j + 1u == end || j + 1u == ori_tiles) mma_commit(sm.bar(kBarQueryEmpty));
             }
-            __syncwarp();
-            if (t && !output_product(t - 1u)) return;
         }
     }
-    if (t) output_product(t - 1u);
+}
+
+// O[128 channels, 128 code rows] = K^T . P for each of the four channel blocks, two blocks in tensor memory.
+__device__ void issue_outputs(const Tree &p, const WalkShared &sm, uint32_t tmem)
+{
+    constexpr uint32_t kOut = idesc_i8(128, kCodeRows, 1, 1);
+    const bool leader = elect_one();
+    const uint64_t keys = smem_desc(sm.base + kSmKey, kSeg, 1024u, kSwizzle128), weights = smem_desc(sm.base + kSmWeight, kSeg, 1024u, kSwizzle128);
+    Items<true> it;
+    uint32_t tiles = 0;                                       // only their number matters here
+    for (bool more = it.first(p); more; more = it.advance(p)) tiles += it.end - it.begin;
+    tiles = same(tiles);
+    for (uint32_t t = 0; t < tiles; ++t) {
+        const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
+        if (!walk_wait<3>(sm, kBarWeightReady + buf, ph)) return;
+        const uint64_t a0 = keys + buf * ((4u * kSeg) >> 4), b0 = weights + buf * (kSeg >> 4);
+#pragma unroll
+        for (uint32_t block = 0; block < 4; ++block) {
+            // use 2 t + (block >> 1) of this half of the output columns
+            if (!walk_wait<3>(sm, kBarOutFree + (block & 1u), ((block >> 1) & 1u) ^ 1u)) return;
+            tc_fence_after();
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+                if (leader) mma_i8(tmem + kColOut + (block & 1u) * kCodeRows, a0 + ((block * kSeg + k * 4096u) >> 4), b0 + ((k * 4096u) >> 4), kOut, k);
+            if (leader) {
+                mma_commit(sm.bar(kBarOutFull + (block & 1u)));
+                // the last reader of two segments, and with the second two of the weights
+                if (block & 1u) mma_commit(sm.bar(kBarKeyEmpty + 2u * buf + (block >> 1)));
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------------ walk: softmax (warps 0-7)
@@ -718,7 +764,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
     uint32_t phase = 0, t = 0, vote = kFlagVote + half * 3u;
     if (key < kRows) top[key] = INT32_MIN;
 
-    Items it;
+    Items<false> it;
     uint32_t items = 0;
     for (bool more = it.first(p); more; more = it.advance(p), ++items) {
         const uint32_t row0 = half * kRows;                   // first row of the half in the group
@@ -731,7 +777,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 const float *alphas = reinterpret_cast<const float *>(p.at(p.s.alphas));
                 alpha[key] = mine ? __ldcg(alphas + row) : 0.f;
                 alpha[kGroupRows + key] = mine && p.s.kinds == 2u ? __ldcg(alphas + (uint64_t)p.s.octets * kOctet + row) : 0.f;
-                ref[key] = kNoKey;
+                ref[key] = -kNoKey;
             } else if (key < kRows + kOctets) {
                 const uint32_t o = half * kOctets + key - kRows;
                 uint64_t m = 0, c = 0;
@@ -790,108 +836,120 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             }
 
             if (!walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
-            if (t >= 2u && !walk_wait<0>(sm, kBarWeightFree + buf, ph ^ 1u)) return;
+            // the weights of tile t - 2 have been read when its last two key segments have
+            if (t >= 2u && !walk_wait<0>(sm, kBarKeyEmpty + 2u * buf + 1u, ph ^ 1u)) return;
             tc_fence_after();
             const float *alpha = sm.floats(kSmAlpha) + row0 + (ori ? 0u : kGroupRows);
             char *weights = sm.ptr + kSmWeight + buf * kSeg + key * 128u;
             const uint32_t columns = score + buf * kCodeRows;
-            // log2 logits of octet o: integers joined exactly, one conversion, one FMA with the offset
-            auto logits = [&](uint32_t o, bool absolute, float (&x)[8]) {
-                uint32_t hi[8], lo[8];
-                tmem_ld8(columns + o * 8u, hi);
-                tmem_ld8(columns + kGroupRows + o * 8u, lo);
-                float bias = 0.f;
+            // log2 of how often octet o counts this key: minus infinity where it does not see it
+            auto bias_of = [&](uint32_t o) {
+                float bias = (sees >> o) & 1u ? 0.f : -INFINITY;
                 if (LISTED) {
                     const uint32_t n = ((o & 2u ? count.y : count.x) >> ((o & 1u) * 16u)) & 0xffffu;
-                    if (n > 1u) bias = log2f((float)n);
+                    if (n > 1u && bias == 0.f) bias = log2f((float)n);
                 }
-                const bool seen = (sees >> o) & 1u;
-                tmem_wait_ld();
+                return bias;
+            };
+            // One octet: integers joined exactly and converted once, log2 weights by packed FMAs, codes, their sums over
+            // the warp, and the codes' bytes to shared memory.  Returns the largest log2 weight.
+            uint32_t total = 0;
+            auto codes = [&](uint32_t o, const uint32_t *hi, const uint32_t *lo) {
+                const float bias = bias_of(o);
+                const uint64_t bias2 = pack2(bias, bias), steps = pack2(kWeightSteps, kWeightSteps), magic = pack2(8388736.f, 8388736.f);
+                uint32_t d[8], sum[8];
+                float most = -INFINITY;
 #pragma unroll
-                for (uint32_t q = 0; q < 2; ++q) {
-                    const float4 a = reinterpret_cast<const float4 *>(alpha)[o * 2u + q], m = reinterpret_cast<const float4 *>(ref)[o * 2u + q];
-                    const float as[4] = {a.x, a.y, a.z, a.w}, ms[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const float off = absolute ? bias : LISTED ? bias - ms[i] : -ms[i];
-                        const float v = fmaf((float)((int32_t)hi[4 * q + i] * 254 + (int32_t)lo[4 * q + i]), as[i], off);
-                        x[4 * q + i] = seen ? v : -INFINITY;
-                    }
+                for (uint32_t q = 0; q < 4; ++q) {
+                    const uint64_t a = reinterpret_cast<const uint64_t *>(alpha)[o * 4u + q], off = add2(reinterpret_cast<const uint64_t *>(ref)[o * 4u + q], bias2);
+                    const uint64_t x = fma2(pack2((float)((int32_t)hi[2 * q] * 254 + (int32_t)lo[2 * q]),
+                                                  (float)((int32_t)hi[2 * q + 1] * 254 + (int32_t)lo[2 * q + 1])), a, off);
+                    const float x0 = low2(x), x1 = high2(x);
+                    most = fmaxf(most, fmaxf(x0, x1));
+                    const uint64_t c = fma2(pack2(exp2_approx(x0), exp2_approx(x1)), steps, magic);      // 2^23 + 128 + code
+                    d[2 * q] = __float_as_uint(low2(c));
+                    d[2 * q + 1] = __float_as_uint(high2(c));
                 }
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) sum[i] = __reduce_add_sync(0xffffffffu, d[i]);
+                const uint32_t chunk = half * 2u + (o >> 1), place = (o & 1u) * 8u;
+                *reinterpret_cast<uint2 *>(weights + ((chunk ^ (key & 7u)) << 4) + place) =
+                    make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410),
+                               __byte_perm(__byte_perm(d[4], d[5], 0x0051), __byte_perm(d[6], d[7], 0x0051), 0x5410));
+                *reinterpret_cast<uint2 *>(weights + (((4u + chunk) ^ (key & 7u)) << 4) + place) =
+                    make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0040), __byte_perm(d[2], d[3], 0x0040), 0x5410) ^ 0x80808080u,
+                               __byte_perm(__byte_perm(d[4], d[5], 0x0040), __byte_perm(d[6], d[7], 0x0040), 0x5410) ^ 0x80808080u);
+                // lane 8 o + i keeps the sum of row i
+                const uint32_t s01 = lane & 1u ? sum[1] : sum[0], s23 = lane & 1u ? sum[3] : sum[2], s45 = lane & 1u ? sum[5] : sum[4], s67 = lane & 1u ? sum[7] : sum[6];
+                const uint32_t s03 = lane & 2u ? s23 : s01, s47 = lane & 2u ? s67 : s45, s = lane & 4u ? s47 : s03;
+                if ((lane >> 3) == o) total = s - 32u * kCodeBias;
+                return most;
             };
             // The first tile of an item has no references to start from.
-            uint32_t todo = j == it.begin ? 0u : 0xfu, total = 0;
-            bool again = false;
-            for (;;) {
+            uint32_t todo = 0xfu;
+            if (j != it.begin) {
                 uint32_t above = 0;
 #pragma unroll 1
-                for (uint32_t o = 0; o < kOctets; ++o) {
-                    if (!((todo >> o) & 1u)) continue;
-                    float x[8];
-                    logits(o, false, x);
-                    const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-                    above |= most > 0.f ? 1u << o : 0u;
-                    uint32_t d[8];
-                    const uint32_t at = lane - o * 8u;
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i) {
-                        d[i] = __float_as_uint(__fmaf_rn(exp2_approx(x[i]), kWeightSteps, 8388736.f));     // 2^23 + 128 + code
-                        const uint32_t sum = __reduce_add_sync(0xffffffffu, d[i]);
-                        if (at == i) total = sum - 32u * kCodeBias;
-                    }
-                    const uint32_t chunk = half * 2u + (o >> 1), place = (o & 1u) * 8u;
-                    *reinterpret_cast<uint2 *>(weights + ((chunk ^ (key & 7u)) << 4) + place) =
-                        make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410),
-                                   __byte_perm(__byte_perm(d[4], d[5], 0x0051), __byte_perm(d[6], d[7], 0x0051), 0x5410));
-                    *reinterpret_cast<uint2 *>(weights + (((4u + chunk) ^ (key & 7u)) << 4) + place) =
-                        make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0040), __byte_perm(d[2], d[3], 0x0040), 0x5410) ^ 0x80808080u,
-                                   __byte_perm(__byte_perm(d[4], d[5], 0x0040), __byte_perm(d[6], d[7], 0x0040), 0x5410) ^ 0x80808080u);
+                for (uint32_t o = 0; o < kOctets; o += 2) {   // two octets at a time, for loads and arithmetic to overlap
+                    uint32_t hi[16], lo[16];
+                    tmem_ld16(columns + o * 8u, hi);
+                    tmem_ld16(columns + kGroupRows + o * 8u, lo);
+                    tmem_wait_ld();
+                    const float first = codes(o, hi, lo), second = codes(o + 1u, hi + 8, lo + 8);
+                    above |= (first > 0.f ? 1u << o : 0u) | (second > 0.f ? 2u << o : 0u);
                 }
-                if (again) break;
-                if (j == it.begin) {
-                    todo = 0xfu;
-                } else {
-                    if (above) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
-                    if (!softmax_sync(sm, half, phase)) return;
-                    todo = flags[vote];
-                    const uint32_t first = kFlagVote + half * 3u;
-                    vote = vote == first + 2u ? first : vote + 1u;
-                    // the word after next was last read before the barrier just passed, and is set behind the next one
-                    if (key == 0) flags[vote == first + 2u ? first : vote + 1u] = 0;
-                }
-                if (key == 0) flags[kFlagRescale + buf * 2u + half] = todo;
-                if (!todo) break;
+                if (above) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
+                if (!softmax_sync(sm, half, phase)) return;
+                todo = flags[vote];
+                const uint32_t zero = kFlagVote + half * 3u;
+                vote = vote == zero + 2u ? zero : vote + 1u;
+                // the word after next was last read before the barrier just passed, and is set behind the next one
+                if (key == 0) flags[vote == zero + 2u ? zero : vote + 1u] = 0;
+            }
+            if (key == 0) flags[kFlagRescale + buf * 2u + half] = todo;
+            if (todo) {
                 // exact row maxima of the octets concerned: integers in float order
                 int32_t high = INT32_MIN;
 #pragma unroll 1
                 for (uint32_t o = 0; o < kOctets; ++o) {
                     if (!((todo >> o) & 1u)) continue;
-                    float x[8];
-                    logits(o, true, x);
-                    const uint32_t at = lane - o * 8u;
+                    uint32_t hi[8], lo[8];
+                    tmem_ld8(columns + o * 8u, hi);
+                    tmem_ld8(columns + kGroupRows + o * 8u, lo);
+                    const float bias = bias_of(o);
+                    tmem_wait_ld();
 #pragma unroll
                     for (uint32_t i = 0; i < 8; ++i) {
-                        const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x[i])));
-                        if (at == i) high = v;
+                        const float x = fmaf((float)((int32_t)hi[i] * 254 + (int32_t)lo[i]), alpha[o * 8u + i], bias);
+                        const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x)));
+                        if (lane == o * 8u + i) high = v;
                     }
                 }
                 atomicMax(top + lane, high);
                 if (!softmax_sync(sm, half, phase)) return;
                 float *factors = sm.floats(kSmFactor) + buf * kGroupRows + row0;
                 if (key < kRows) {
-                    const float highest = __int_as_float(ordered(top[key])), old = ref[key];
+                    const float highest = __int_as_float(ordered(top[key])), old = -ref[key];
                     float now = old, factor = 1.f;
                     if (highest > old - 1.f) {                // the margin covers the rounding of x; a NaN moves nothing
                         now = highest + kHeadroom;
                         factor = exp2_approx(old - now);
                     }
                     top[key] = INT32_MIN;
-                    ref[key] = now;
+                    ref[key] = -now;
                     factors[key] = factor;
                 }
                 if (!softmax_sync(sm, half, phase)) return;
                 row_sum *= factors[lane];
-                again = true;
+#pragma unroll 1
+                for (uint32_t o = 0; o < kOctets; ++o) {
+                    if (!((todo >> o) & 1u)) continue;
+                    uint32_t hi[8], lo[8];
+                    tmem_ld8(columns + o * 8u, hi);
+                    tmem_ld8(columns + kGroupRows + o * 8u, lo);
+                    tmem_wait_ld();
+                    codes(o, hi, lo);
+                }
             }
             tc_fence_before();
             mbar_arrive(sm.bar(kBarScoreFree + buf));
@@ -909,7 +967,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
         if (!walk_wait<0>(sm, kBarDoneFree, (items & 1u) ^ 1u)) return;
         if (mine) {
             const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
-            const float a = sm.floats(kSmAlpha)[row0 + key], l = a != a ? a : sums[key], m = ref[key];      // NaN: a query row that is not finite
+            const float a = sm.floats(kSmAlpha)[row0 + key], l = a != a ? a : sums[key], m = -ref[key];      // NaN: a query row that is not finite
             if (it.whole()) {
                 const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
                 const float sink2 = sink * kLog2e, at = fmaxf(m, sink2), own = exp2_approx(m - at);
@@ -936,14 +994,14 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
 {
     const uint32_t index = threadIdx.x - kWarpAccumulate * 32u, h = index >> 7, channel = index & 127u, warp = channel >> 5;
     const uint32_t tmem_lane = tmem + ((warp * 32u) << 16) + kColOut + h * 32u;
-    Items it;
+    Items<false> it;
     uint32_t t = 0, items = 0;
     for (bool more = it.first(p); more; more = it.advance(p), ++items) {
-        float acc[4][32];
+        uint64_t acc[4][16];                                  // pairs of rows
 #pragma unroll
         for (int block = 0; block < 4; ++block)
 #pragma unroll
-            for (int r = 0; r < 32; ++r) acc[block][r] = 0.f;
+            for (int r = 0; r < 16; ++r) acc[block][r] = 0;
         for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
             const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
             if (!walk_wait<1>(sm, kBarWeightReady + buf, ph)) return;
@@ -953,18 +1011,23 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     const float units = __ldg(reinterpret_cast<const float *>(p.a.oriScale) + block * 128 + channel) /
                                         __ldg(reinterpret_cast<const float *>(p.a.cmpScale) + block * 128 + channel);
 #pragma unroll
-                    for (int r = 0; r < 32; ++r) acc[block][r] *= units;
+                    for (int r = 0; r < 16; ++r) acc[block][r] = mul2(acc[block][r], pack2(units, units));
                 }
             }
-            if (sm.flags()[kFlagRescale + buf * 2u + h]) {
-                const float4 *factor = reinterpret_cast<const float4 *>(sm.ptr + kSmFactor) + buf * 16u + h * 8u;
+            const uint32_t moved = sm.flags()[kFlagRescale + buf * 2u + h];
+            if (moved) {
+                const ulonglong2 *factor = reinterpret_cast<const ulonglong2 *>(sm.ptr + kSmFactor) + buf * 16u + h * 8u;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const float4 f = factor[q];
+                for (int o = 0; o < 4; ++o) {
+                    if (!((moved >> o) & 1u)) continue;
 #pragma unroll
-                    for (int block = 0; block < 4; ++block) {
-                        acc[block][4 * q] *= f.x; acc[block][4 * q + 1] *= f.y;
-                        acc[block][4 * q + 2] *= f.z; acc[block][4 * q + 3] *= f.w;
+                    for (int q = 2 * o; q < 2 * o + 2; ++q) {
+                        const ulonglong2 f = factor[q];
+#pragma unroll
+                        for (int block = 0; block < 4; ++block) {
+                            acc[block][2 * q] = mul2(acc[block][2 * q], f.x);
+                            acc[block][2 * q + 1] = mul2(acc[block][2 * q + 1], f.y);
+                        }
                     }
                 }
             }
@@ -979,12 +1042,15 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     tmem_ld8(tmem_lane + half * kCodeRows + c * 8u, hi);
                     tmem_ld8(tmem_lane + half * kCodeRows + kGroupRows + c * 8u, lo);
                     tmem_wait_ld();
+                    if (c == 3) {
+                        tc_fence_before();
+                        mbar_arrive(sm.bar(kBarOutFree + half));
+                    }
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        acc[block][c * 8u + i] += (float)((int32_t)hi[i] * 256 + (int32_t)lo[i]);
+                    for (uint32_t i = 0; i < 4; ++i)
+                        acc[block][c * 4u + i] = add2(acc[block][c * 4u + i], pack2((float)((int32_t)hi[2 * i] * 256 + (int32_t)lo[2 * i]),
+                                                                                    (float)((int32_t)hi[2 * i + 1] * 256 + (int32_t)lo[2 * i + 1])));
                 }
-                tc_fence_before();
-                mbar_arrive(sm.bar(kBarOutFree + half));
             }
         }
         if (!walk_wait<1>(sm, kBarDone, items & 1u)) return;
@@ -993,9 +1059,11 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
 #pragma unroll
         for (uint32_t block = 0; block < 4; ++block) {
             const float f = __ldg(scale + block * 128u);
+            const uint64_t f2 = pack2(f, f);
 #pragma unroll
-            for (uint32_t r = 0; r < 32; ++r) acc[block][r] *= f;
+            for (uint32_t r = 0; r < 16; ++r) acc[block][r] = mul2(acc[block][r], f2);
         }
+        auto value = [&](uint32_t block, uint32_t r) { return r & 1u ? high2(acc[block][r / 2u]) : low2(acc[block][r / 2u]); };
         if (it.whole()) {
             const float *inverse = sm.floats(kSmInverse) + h * 32u;
             __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.a.out) + ((uint64_t)it.g.first_octet * kOctet + h * 32u) * kDim + channel;
@@ -1004,16 +1072,16 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 if (h * 32u + r < rows) {
                     const float f = inverse[r];
 #pragma unroll
-                    for (uint32_t block = 0; block < 4; ++block) out[r * kDim + block * 128u] = __float2bfloat16_rn(acc[block][r] * f);
+                    for (uint32_t block = 0; block < 4; ++block) out[r * kDim + block * 128u] = __float2bfloat16_rn(value(block, r) * f);
                 }
             }
         } else {
-            float *mine = reinterpret_cast<float *>(p.at(p.s.partials)) + (uint64_t)it.partial() * kPartial + h * 32u * kDim + channel;
+            float *partial = reinterpret_cast<float *>(p.at(p.s.partials)) + (uint64_t)it.partial() * kPartial + h * 32u * kDim + channel;
 #pragma unroll
             for (uint32_t r = 0; r < 32; ++r)
                 if (h * 32u + r < rows)
 #pragma unroll
-                    for (uint32_t block = 0; block < 4; ++block) mine[r * kDim + block * 128u] = acc[block][r];
+                    for (uint32_t block = 0; block < 4; ++block) partial[r * kDim + block * 128u] = value(block, r);
         }
         mbar_arrive(sm.bar(kBarDoneFree));
     }
@@ -1031,12 +1099,13 @@ __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid
     const uint32_t warp = threadIdx.x >> 5;
     volatile uint32_t *flags = sm.flags();
     if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < kRing; ++i) { mbar_init(sm.bar(kBarKeyFull + i), 1); mbar_init(sm.bar(kBarKeyEmpty + i), 1); }
+        for (uint32_t i = 0; i < kRing; ++i) mbar_init(sm.bar(kBarKeyFull + i), 1);
+        for (uint32_t i = 0; i < kRing / 2u; ++i) mbar_init(sm.bar(kBarKeyEmpty + i), 1);
         mbar_init(sm.bar(kBarQueryFull), 1);
         mbar_init(sm.bar(kBarQueryEmpty), 1);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(sm.bar(kBarScoreFull + i), 1); mbar_init(sm.bar(kBarScoreFree + i), 256);
-            mbar_init(sm.bar(kBarWeightReady + i), 256); mbar_init(sm.bar(kBarWeightFree + i), 1);
+            mbar_init(sm.bar(kBarWeightReady + i), 256);
             mbar_init(sm.bar(kBarOutFull + i), 1); mbar_init(sm.bar(kBarOutFree + i), 256);
         }
         mbar_init(sm.bar(kBarSync), 128);
@@ -1065,7 +1134,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid
         accumulate(p, sm, tmem);
     } else {
         registers_release<kRegsIssue>();
-        if (warp == kWarpIssue) issue(p, sm, tmem);
+        if (warp == kWarpIssue) issue_scores(p, sm, tmem);
+        else if (warp == kWarpIssue + 1u) issue_outputs(p, sm, tmem);
         else produce<LISTED>(p, sm, warp - kWarpProduce, &ori_map, &cmp_map, &row_map, gather != 0);
         __syncwarp();
     }

@@ -5,8 +5,8 @@ The kernel's arithmetic errors, for one query row (A = largest |q_c scale_c|, co
 w = e^(s - max s), n keys):
   query codes      two INT8 planes: |dq_c| <= A / (2 * 127 * 254), so |ds| <= Es = softmax_scale * A / 64516 * max_k sum_c |code|
                    and a weight is off by a factor of at most e^(2 Es) once the maximum moves with it;
-  weight codes     steps of 4 / 32639 of the largest weight, the 4 because the reference point may stand
-                   two powers of two above the largest logit: |dw| <= Ew = 2 / 32639;
+  weight codes     steps of 8 / 32639 of the largest weight, the 8 because the reference point may stand
+                   three powers of two above the largest logit; rounded to nearest: |dw| <= Ew = 4 / 32639;
   output           dw moves numerator and denominator: |dy| <= (sum dw |v| + |y| sum dw) / sum w, then one
                    rounding to BF16, half a step: 2^-8 |y|; FP32 sums of the integer products add 2^-20 relative;
   LSE              Es + n Ew / sum w, and 2^-20 of its magnitude in FP32.
@@ -131,7 +131,7 @@ def expected(case, paths, cmp_paths, ori_scale, cmp_scale):
             lse[t] = (top + total.log())[:, 0]
             es = max(float((q * sc).abs().amax() * c.abs().sum(1).amax()) for c, sc in zip(codes, scales) if len(c)) * case.softmax_scale / 64516
             largest = (s.amax(1, keepdim=True) - top).exp()            # weight codes count from the largest logit, not from the sink
-            ew = 2 / 32639 * largest
+            ew = 4 / 32639 * largest
             dw = w * (math.exp(2 * es) - 1) + ew
             out_bound[t] = (dw @ v.abs() + out[t].abs() * dw.sum(1, keepdim=True)) / total + out[t].abs() * (BF16_HALF_STEP + 2 ** -20) + 1e-30
             lse_bound[t] = es + (len(v) * ew / total)[:, 0] + lse[t].abs() * 2 ** -20 + 2 ** -20
