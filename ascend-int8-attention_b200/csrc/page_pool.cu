@@ -2,14 +2,19 @@
 // their page numbering, changed on the device (resize, fork), and the page and row moves that go with
 // them (copy, keep).  The contract is in include/sharedkv_c_abi.h.
 //
-// resize and fork are a plan kernel and a copy kernel.  The plan updates the counts of what is
-// released and shared, finds the lowest-numbered free pages by counting zeros per warp chunk and
-// adding the counts up, checks that they suffice (if not, the count changes are taken back), deals
-// them out in sequence order by a prefix sum and leaves the list of pages to copy in the workspace.
-// Counts change by integer atomics, whose sum does not depend on their order; every other value is
-// written by one thread.
+// resize and fork are planned by one cluster of eight thread blocks (one block for small pools), whose
+// hardware barrier separates the phases: the counts of what is released and shared are updated; zeros are counted per warp chunk and the
+// counts added up, which ranks the lowest-numbered free pages; if they do not suffice the count changes are
+// taken back; else they are dealt out in sequence order by a prefix sum.  Counts change by integer
+// atomics, whose sum does not depend on their order; every other value is written by one thread.
+// The plan is a chain of dependent L2 accesses, so it is bound by latency: one block took 126 us for a
+// fork of 512 sequences of 85 pages, most of it one warp after another waiting for table and counts.
+// Pages are copied by a kernel of their own, over all SMs, or by the plan's blocks where that is at
+// most kPlanCopyBytes (always for resize, which copies only shared, partly filled last pages).
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
 
 #include "../../include/sharedkv_c_abi.h"
 #include "ptx_sm100.cuh"
@@ -21,10 +26,12 @@ namespace {
 using ptx::grid_dependency_launch_dependents;
 using ptx::grid_dependency_wait;
 
-constexpr uint32_t kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
+constexpr uint32_t kPlanBlocks = 8, kPlanThreads = 1024, kBlockWarps = kPlanThreads / 32;
+constexpr uint32_t kAloneWork = 8192;               // pages + table entries up to which one block is as fast as a cluster
 constexpr uint32_t kMaxSequences = 8192;            // rows whose bookkeeping fits the plan kernel's shared memory
 constexpr uint32_t kStripWords = 16384;             // table entries a fork holds in shared memory at a time
 constexpr uint32_t kCopyThreads = 256;
+constexpr uint64_t kPlanCopyBytes = 1u << 20;        // a second launch costs about what eight blocks need for this much
 constexpr uint32_t kCopyUnit = 8192;                // bytes a thread block moves at a time: two 16-byte loads per thread in flight
 constexpr uint32_t kKeepThreads = 256, kMaxKept = 64;
 
@@ -37,6 +44,8 @@ __host__ __device__ constexpr uint64_t page_ws_bytes(uint32_t batch, uint32_t wi
     return page_ws_fresh(batch) + 4ull * batch * ((uint64_t)width + 1ull);
 }
 
+static_assert(kWsCounts + 4 * kPlanBlocks * kBlockWarps <= kWsCopies, "a count per warp");
+
 struct Pool {
     const uint64_t *caches;
     int32_t *table, *lens, *refs;
@@ -44,7 +53,17 @@ struct Pool {
     int2 *copies;
     int32_t *fresh;
     uint32_t layers, pages, rows, batch, width;
+    uint32_t copies_here;          // the plan's blocks copy the pages
 };
+
+// Barrier of the plan's blocks; orders their memory accesses too.
+template <uint32_t BLOCKS>
+__device__ __forceinline__ void plan_sync()
+{
+    if (BLOCKS == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t plan_warp() { return blockIdx.x * kBlockWarps + (threadIdx.x >> 5); }
 
 __device__ __forceinline__ uint32_t pages_of(int32_t rows, uint32_t per_page) { return rows <= 0 ? 0u : ((uint32_t)rows + per_page - 1u) / per_page; }
 
@@ -113,23 +132,45 @@ __device__ __forceinline__ void add_ref(const Pool &p, int32_t page, int32_t del
     if ((uint32_t)page < p.pages) atomicAdd(p.refs + page, delta);
 }
 
-// Finds the `total` lowest free pages; false (for every thread) when there are fewer.
+// Finds the `total` lowest free pages; false (for every thread of the cluster) when there are fewer.
+template <uint32_t BLOCKS>
 __device__ bool take_free(const Pool &p, uint32_t total, uint32_t *scratch)
 {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t chunk = ((p.pages + kPlanWarps - 1u) / kPlanWarps + 31u) & ~31u;
+    constexpr uint32_t kWarps = BLOCKS * kBlockWarps;
+    const uint32_t lane = threadIdx.x & 31u, warp = plan_warp();
+    const uint32_t chunk = ((p.pages + kWarps - 1u) / kWarps + 31u) & ~31u;
     const uint32_t begin = min(warp * chunk, p.pages), end = min(begin + chunk, p.pages);
     const uint32_t mine = count_free(p, begin, end, lane);
-    if (lane == 0) scratch[warp] = mine;
-    __syncthreads();
-    const uint32_t other = scratch[lane];
-    const uint32_t all = __reduce_add_sync(0xffffffffu, other);
-    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0u);
+    if (lane == 0) p.counts[warp] = mine;
+    plan_sync<BLOCKS>();
+    uint32_t all = 0, before = 0;
+#pragma unroll
+    for (uint32_t i = lane; i < kWarps; i += 32u) {
+        const uint32_t n = __ldcg(p.counts + i);
+        all += n;
+        before += i < warp ? n : 0u;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    before = __reduce_add_sync(0xffffffffu, before);
     if (all >= total) list_free(p, begin, end, before, total, lane);
-    __syncthreads();
+    plan_sync<BLOCKS>();
     return all >= total;
 }
 
+// Copies up to four rows of a page in one cache (one warp).
+__device__ __forceinline__ void copy_rows(const Pool &p, uint32_t layer, int32_t source, int32_t target, uint32_t first, uint32_t count, uint32_t lane)
+{
+    const uint64_t base = p.caches[2u * layer], stride = p.caches[2u * layer + 1u];
+    const uint4 *src = reinterpret_cast<const uint4 *>(base + (uint64_t)source * stride) + first * 32u + lane;
+    uint4 *dst = reinterpret_cast<uint4 *>(base + (uint64_t)target * stride) + first * 32u + lane;
+    uint4 v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) if (k < count) v[k] = src[k * 32u];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) if (k < count) dst[k * 32u] = v[k];
+}
+
+template <uint32_t BLOCKS>
 __global__ void __launch_bounds__(kPlanThreads, 1) page_resize_plan(const Pool p, const int32_t *wanted)
 {
     extern __shared__ uint32_t smem[];
@@ -137,23 +178,23 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_resize_plan(const Pool p
     __shared__ uint32_t scratch[64];
     grid_dependency_launch_dependents();
     grid_dependency_wait();
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    constexpr uint32_t kWarps = BLOCKS * kBlockWarps;
+    const uint32_t lane = threadIdx.x & 31u, warp = plan_warp();
     bool bad = false;
     for (uint32_t b = threadIdx.x; b < p.batch; b += kPlanThreads)
         bad |= wanted[b] < 0 || pages_of(wanted[b], p.rows) > p.width || pages_of(p.lens[b], p.rows) > p.width;
-    if (threadIdx.x == 0) p.head[1] = 0;
-    if (__syncthreads_or(bad)) {
+    if (__syncthreads_or(bad)) {                              // the same in every block
         if (threadIdx.x == 0) p.head[0] = kStatusRange;
         return;
     }
     auto release = [&](int32_t delta) {
-        for (uint32_t b = warp; b < p.batch; b += kPlanWarps) {
+        for (uint32_t b = warp; b < p.batch; b += kWarps) {
             const uint32_t before = pages_of(p.lens[b], p.rows), after = pages_of(wanted[b], p.rows);
-            for (uint32_t k = after + lane; k < before; k += 32u) add_ref(p, p.table[(uint64_t)b * p.width + k], delta);
+            for (uint32_t k = after + lane; k < before; k += 32u) add_ref(p, __ldcg(p.table + (uint64_t)b * p.width + k), delta);
         }
     };
     release(-1);
-    __syncthreads();
+    plan_sync<BLOCKS>();
     for (uint32_t b = threadIdx.x; b < p.batch; b += kPlanThreads) {
         const uint32_t before = pages_of(p.lens[b], p.rows), after = pages_of(wanted[b], p.rows);
         uint32_t need = after > before ? after - before : 0u;
@@ -165,22 +206,26 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_resize_plan(const Pool p
     }
     __syncthreads();
     const uint32_t total = scan_sequences(offset, p.batch, scratch);
-    if (!take_free(p, total, scratch)) {
+    if (!take_free<BLOCKS>(p, total, scratch)) {
         release(1);
         if (threadIdx.x == 0) p.head[0] = kStatusRange;
         return;
     }
-    for (uint32_t b = warp; b < p.batch; b += kPlanWarps) {
+    for (uint32_t b = warp; b < p.batch; b += kWarps) {
         const uint32_t before = pages_of(p.lens[b], p.rows), after = pages_of(wanted[b], p.rows);
         const uint32_t first = offset[b], count = (b + 1u < p.batch ? offset[b + 1u] : total) - first;
         const uint32_t grown = after > before ? after - before : 0u, split = count - grown;      // split: 1 when the last page is replaced
         int32_t *row = p.table + (uint64_t)b * p.width;
-        if (split && lane == 0) {
+        if (split) {
             const int32_t source = row[before - 1u], page = p.fresh[first];
-            row[before - 1u] = page;
-            p.refs[page] = 1;
-            atomicAdd(p.refs + source, -1);
-            p.copies[atomicAdd(p.head + 1, 1u)] = make_int2(source, page);
+            __syncwarp();
+            if (lane == 0) {
+                row[before - 1u] = page;
+                p.refs[page] = 1;
+                atomicAdd(p.refs + source, -1);
+            }
+            for (uint32_t layer = 0; layer < p.layers; ++layer)
+                for (uint32_t r = 0; r < p.rows; r += 4u) copy_rows(p, layer, source, page, r, min(p.rows - r, 4u), lane);
         }
         for (uint32_t k = lane; k < grown; k += 32u) {
             const int32_t page = p.fresh[first + split + k];
@@ -192,6 +237,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_resize_plan(const Pool p
     }
 }
 
+template <uint32_t BLOCKS>
 __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, const int32_t *parents)
 {
     extern __shared__ uint32_t smem[];
@@ -202,7 +248,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
     __shared__ uint32_t scratch[64];
     grid_dependency_launch_dependents();
     grid_dependency_wait();
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    constexpr uint32_t kWarps = BLOCKS * kBlockWarps;
+    const uint32_t lane = threadIdx.x & 31u, warp = plan_warp();
     bool bad = false;
     uint32_t longest = 0;
     for (uint32_t b = threadIdx.x; b < p.batch; b += kPlanThreads) {
@@ -212,7 +259,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
         first[b] = 0xffffffffu;
         bad |= parents[b] >= (int32_t)p.batch || pages_of(len[b], p.rows) > p.width;
     }
-    if (threadIdx.x == 0) { p.head[1] = 0; scratch[40] = 0; }
+    if (threadIdx.x == 0) scratch[40] = 0;
+    if (threadIdx.x == 0 && blockIdx.x == 0) p.head[1] = 0;
     if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0) p.head[0] = kStatusRange;
         return;
@@ -230,7 +278,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
         offset[b] = parent[b] >= 0 && first[parent[b]] != b && len[parent[b]] > 0 && (uint32_t)len[parent[b]] % p.rows != 0;
     // full pages gain a reference per further child; a sequence without a child gives up all of its pages
     auto share = [&](int32_t sign) {
-        for (uint32_t b = warp; b < p.batch; b += kPlanWarps) {
+        for (uint32_t b = warp; b < p.batch; b += kWarps) {
             if (children[b] == 1) continue;
             const uint32_t live = pages_of(len[b], p.rows), full = len[b] <= 0 ? 0u : (uint32_t)len[b] / p.rows;
             for (uint32_t k = lane; k < (children[b] ? full : live); k += 32u)
@@ -238,19 +286,20 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
         }
     };
     share(1);
-    __syncthreads();
+    plan_sync<BLOCKS>();
     const uint32_t total = scan_sequences(offset, p.batch, scratch);
-    if (!take_free(p, total, scratch)) {
+    if (!take_free<BLOCKS>(p, total, scratch)) {
         share(-1);
         if (threadIdx.x == 0) p.head[0] = kStatusRange;
         return;
     }
-    // The table is permuted in place, a strip of columns at a time: all rows of the strip are read
-    // before one is written.
+    // The table is permuted in place, a strip of columns at a time, the strips dealt to the blocks: all rows of
+    // a strip are read before one is written.
     uint32_t columns = 32;
     while (columns > 1u && columns * p.batch > kStripWords) columns >>= 1;
+    while (columns > 8u && columns * BLOCKS > longest) columns >>= 1;         // a strip for every block, but whole 32-byte sectors
     const uint32_t cells = columns * p.batch, shift = 31u - __clz(columns);
-    for (uint32_t left = 0; left < longest; left += columns) {
+    for (uint32_t left = blockIdx.x * columns; left < longest; left += BLOCKS * columns) {
         for (uint32_t i = threadIdx.x; i < cells; i += kPlanThreads) {
             const uint32_t b = i >> shift, k = left + (i & (columns - 1u));
             if (k < pages_of(len[b], p.rows)) strip[i] = p.table[(uint64_t)b * p.width + k];
@@ -276,7 +325,18 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
         }
         __syncthreads();
     }
-    for (uint32_t b = threadIdx.x; b < p.batch; b += kPlanThreads) p.lens[b] = parent[b] < 0 ? 0 : len[parent[b]];
+    if (blockIdx.x == 0)                                      // every block has had its own copy since before the first barrier
+        for (uint32_t b = threadIdx.x; b < p.batch; b += kPlanThreads) p.lens[b] = parent[b] < 0 ? 0 : len[parent[b]];
+    if (p.copies_here) {
+        plan_sync<BLOCKS>();
+        const uint32_t count = __ldcg(p.head + 1);
+        const uint32_t pieces = (p.rows + 3u) / 4u;           // a warp moves four rows of one cache at a time
+        for (uint32_t i = warp; i < count * p.layers * pieces; i += kWarps) {
+            const uint32_t piece = i % pieces, layer = i / pieces % p.layers;
+            const int2 pair = __ldcg(p.copies + i / pieces / p.layers);
+            if ((uint32_t)pair.x < p.pages) copy_rows(p, layer, pair.x, pair.y, piece * 4u, min(p.rows - piece * 4u, 4u), lane);
+        }
+    }
 }
 
 // Page copies: unit = 8 KB of one page of one cache; thread blocks walk the units in order.  Streaming:
@@ -307,58 +367,93 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const uint64_t 
     }
 }
 
-// One thread block per (sequence, layer): a warp takes kept rows w, w + 8, ...; every row (32 lanes x 16
-// bytes) is in registers before the block-wide barrier, and written behind it.
-__global__ void __launch_bounds__(kKeepThreads) page_keep_kernel(const Pool p, const int32_t *base, const int32_t *kept, uint32_t kept_width)
+// A thread block takes a sequence in some of the layers: where the rows come from and go to is looked up
+// once.  A warp takes kept rows w, w + 8, ...; of kKeepLayers layers at a time, every row (32 lanes x 16 bytes)
+// is in registers before the block-wide barrier, and written behind it.  Bound by the latency of the look-ups for
+// small trees, by HBM for many layers.
+template <uint32_t ROUNDS>
+__global__ void __launch_bounds__(kKeepThreads) page_keep_kernel(const Pool p, const int32_t *base, const int32_t *kept, uint32_t kept_width,
+                                                                 uint32_t layers_per_block)
 {
+    constexpr uint32_t kWarps = kKeepThreads / 32, kKeepLayers = ROUNDS <= 2 ? 4 : 2;
     grid_dependency_launch_dependents();
     grid_dependency_wait();
-    constexpr uint32_t kWarps = kKeepThreads / 32, kRounds = kMaxKept / kWarps;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    for (uint64_t item = blockIdx.x; item < (uint64_t)p.batch * p.layers; item += gridDim.x) {
-        const uint32_t b = (uint32_t)(item / p.layers), layer = (uint32_t)(item % p.layers);
-        const uint64_t cache = p.caches[2u * layer], stride = p.caches[2u * layer + 1u];
+    const uint32_t groups = (p.layers + layers_per_block - 1u) / layers_per_block;
+    for (uint64_t item = blockIdx.x; item < (uint64_t)p.batch * groups; item += gridDim.x) {
+        const uint32_t b = (uint32_t)(item / groups), first = (uint32_t)(item % groups) * layers_per_block;
+        const uint32_t last = min(first + layers_per_block, p.layers);
         const int32_t start = base[b];
-        auto address = [&](int64_t row) -> uint64_t {           // of a logical row; 0 when it has no page
-            if (row < 0 || row >= (int64_t)p.width * p.rows) return 0;
-            const int32_t page = p.table[(uint64_t)b * p.width + (uint32_t)(row / p.rows)];
-            return (uint32_t)page < p.pages ? cache + (uint64_t)page * stride + (uint64_t)(row % p.rows) * 512u : 0ull;
-        };
-        uint4 v[kRounds];
-        uint64_t target[kRounds];
-#pragma unroll
-        for (uint32_t r = 0; r < kRounds; ++r) {
-            const uint32_t i = r * kWarps + warp;
-            target[r] = 0;
-            if (i >= kept_width) continue;
-            const int32_t from = kept[(uint64_t)b * kept_width + i];
-            if (from < 0 || (uint32_t)from == i) continue;      // a row that is in its place already
-            const uint64_t source = address((int64_t)start + from), to = address((int64_t)start + i);
-            if (!source || !to) continue;
-            v[r] = *reinterpret_cast<const uint4 *>(source + lane * 16u);
-            target[r] = to;
+        // lane r looks up round r: page and row of source and target
+        int32_t from_page = -1, to_page = -1;
+        uint32_t from_row = 0, to_row = 0;
+        if (lane < ROUNDS) {
+            const uint32_t i = lane * kWarps + warp;
+            const int32_t from = i < kept_width ? kept[(uint64_t)b * kept_width + i] : -1;
+            auto place = [&](int64_t row, int32_t &page, uint32_t &in_page) {
+                if (row < 0 || row >= (int64_t)p.width * p.rows) return;
+                page = p.table[(uint64_t)b * p.width + (uint32_t)row / p.rows];
+                in_page = (uint32_t)row % p.rows;
+            };
+            if (from >= 0 && (uint32_t)from != i) {           // others are in their place already
+                place((int64_t)start + from, from_page, from_row);
+                place((int64_t)start + i, to_page, to_row);
+            }
+            if ((uint32_t)from_page >= p.pages || (uint32_t)to_page >= p.pages) to_page = -1;
         }
-        __syncthreads();
+        for (uint32_t layer = first; layer < last; layer += kKeepLayers) {
+            uint4 v[kKeepLayers][ROUNDS];
 #pragma unroll
-        for (uint32_t r = 0; r < kRounds; ++r)
-            if (target[r]) *reinterpret_cast<uint4 *>(target[r] + lane * 16u) = v[r];
-        __syncthreads();
+            for (uint32_t l = 0; l < kKeepLayers; ++l) {
+                if (layer + l >= last) continue;
+                const uint64_t cache = p.caches[2u * (layer + l)], stride = p.caches[2u * (layer + l) + 1u];
+#pragma unroll
+                for (uint32_t r = 0; r < ROUNDS; ++r) {
+                    const int32_t page = __shfl_sync(0xffffffffu, from_page, r);
+                    const uint32_t row = __shfl_sync(0xffffffffu, from_row, r);
+                    if (__shfl_sync(0xffffffffu, to_page, r) >= 0)
+                        v[l][r] = *reinterpret_cast<const uint4 *>(cache + (uint64_t)(uint32_t)page * stride + row * 512ull + lane * 16u);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (uint32_t l = 0; l < kKeepLayers; ++l) {
+                if (layer + l >= last) continue;
+                const uint64_t cache = p.caches[2u * (layer + l)], stride = p.caches[2u * (layer + l) + 1u];
+#pragma unroll
+                for (uint32_t r = 0; r < ROUNDS; ++r) {
+                    const int32_t page = __shfl_sync(0xffffffffu, to_page, r);
+                    const uint32_t row = __shfl_sync(0xffffffffu, to_row, r);
+                    if (page >= 0)
+                        *reinterpret_cast<uint4 *>(cache + (uint64_t)(uint32_t)page * stride + row * 512ull + lane * 16u) = v[l][r];
+                }
+            }
+        }
     }
 }
 
 template <class... Params, class... Args>
-cudaError_t launch(void (*kernel)(Params...), uint32_t blocks, uint32_t threads, uint32_t smem, cudaStream_t stream, Args... args)
+cudaError_t launch(void (*kernel)(Params...), uint32_t cluster, uint32_t blocks, uint32_t threads, uint32_t smem, cudaStream_t stream, Args... args)
 {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(blocks);
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
-    cudaLaunchAttribute attribute[1];
-    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attribute[2];
     config.attrs = attribute;
-    config.numAttrs = programmatic_launch_enabled() ? 1u : 0u;
+    config.numAttrs = 0;
+    if (cluster > 1u) {
+        attribute[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attribute[config.numAttrs].val.clusterDim.x = cluster;
+        attribute[config.numAttrs].val.clusterDim.y = attribute[config.numAttrs].val.clusterDim.z = 1;
+        ++config.numAttrs;
+    }
+    if (programmatic_launch_enabled()) {
+        attribute[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute[config.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++config.numAttrs;
+    }
     return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
 }
 
@@ -368,7 +463,7 @@ cudaError_t launch_copies(const PagePoolArgs &a, const int2 *pairs, const uint32
     const uint64_t units = (uint64_t)most * a.layers * ((page_bytes + kCopyUnit - 1u) / kCopyUnit);
     const uint64_t cap = (uint64_t)sms * 8u;                    // eight 256-thread blocks fill an SM
     const uint32_t blocks = (uint32_t)(units < cap ? units : cap);
-    return launch(page_copy_kernel, blocks, kCopyThreads, 0u, stream, reinterpret_cast<const uint64_t *>(a.caches), pairs, count_word, count,
+    return launch(page_copy_kernel, 1u, blocks, kCopyThreads, 0u, stream, reinterpret_cast<const uint64_t *>(a.caches), pairs, count_word, count,
                   a.layers, a.pages, page_bytes);
 }
 
@@ -405,16 +500,31 @@ int page_plan(uint32_t op, const PagePoolArgs *args, const int32_t *input, cudaS
     p.copies = reinterpret_cast<int2 *>(ws + kWsCopies);
     p.fresh = reinterpret_cast<int32_t *>(ws + page_ws_fresh(a.batch));
     p.layers = a.layers; p.pages = a.pages; p.rows = a.pageRows; p.batch = a.batch; p.width = a.width;
+    // a fork makes fewer copies than it has sequences
+    p.copies_here = (uint64_t)a.batch * a.layers * a.pageRows * 512u <= kPlanCopyBytes;
     cudaError_t e;
+    const bool alone = (uint64_t)a.pages + (uint64_t)a.batch * a.width <= kAloneWork;
+    const uint32_t blocks = alone ? 1u : kPlanBlocks;
     if (op == 0) {
-        e = launch(page_resize_plan, 1u, kPlanThreads, 4u * a.batch, stream, p, input);
-    } else {
-        const uint32_t strip = a.batch > kStripWords ? a.batch : kStripWords;
-        const uint32_t smem = 4u * (4u * a.batch + strip);
-        e = cudaFuncSetAttribute(page_fork_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(4u * (4u * kMaxSequences + kStripWords)));
-        if (e == cudaSuccess) e = launch(page_fork_plan, 1u, kPlanThreads, smem, stream, p, input);
+        const auto kernel = alone ? page_resize_plan<1> : page_resize_plan<kPlanBlocks>;
+        return (int)launch(kernel, blocks, blocks, kPlanThreads, 4u * a.batch, stream, p, input);
     }
-    if (e == cudaSuccess) e = launch_copies(a, p.copies, p.head + 1, 0u, a.batch, sms, stream);
+    const uint32_t strip = a.batch > kStripWords ? a.batch : kStripWords;
+    const auto kernel = alone ? page_fork_plan<1> : page_fork_plan<kPlanBlocks>;
+    static std::atomic<uint64_t> configured{0};               // opt-in to large dynamic shared memory, per device
+    int device = 0;
+    e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return (int)e;
+    const uint64_t bit = device >= 0 && device < kMaxDevices ? 1ull << device : 0ull;
+    if (!bit || !(configured.load(std::memory_order_relaxed) & bit)) {
+        constexpr int kMost = (int)(4u * (4u * kMaxSequences + kStripWords));
+        e = cudaFuncSetAttribute(page_fork_plan<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(page_fork_plan<kPlanBlocks>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        if (e != cudaSuccess) return (int)e;
+        configured.fetch_or(bit, std::memory_order_relaxed);
+    }
+    e = launch(kernel, blocks, blocks, kPlanThreads, 4u * (4u * a.batch + strip), stream, p, input);
+    if (e == cudaSuccess && !p.copies_here) e = launch_copies(a, p.copies, p.head + 1, 0u, a.batch, sms, stream);
     return (int)e;
 }
 
@@ -442,8 +552,14 @@ int page_keep(const PagePoolArgs *args, const int32_t *base, const int32_t *kept
     p.caches = reinterpret_cast<const uint64_t *>(a.caches);
     p.table = reinterpret_cast<int32_t *>(a.table);
     p.layers = a.layers; p.pages = a.pages; p.rows = a.pageRows; p.batch = a.batch; p.width = a.width;
-    const uint64_t items = (uint64_t)a.batch * a.layers, cap = (uint64_t)sms * 8u;
-    return (int)launch(page_keep_kernel, (uint32_t)(items < cap ? items : cap), kKeepThreads, 0u, stream, p, base, kept, kept_width);
+    // Layers share the look-ups; a block takes as few of them as still give every SM eight blocks.
+    const uint64_t cap = (uint64_t)sms * 8u;
+    uint32_t per_block = (uint32_t)(((uint64_t)a.batch * a.layers + cap - 1u) / cap);
+    per_block = per_block < a.layers ? (per_block ? per_block : 1u) : a.layers;
+    const uint64_t items = (uint64_t)a.batch * ((a.layers + per_block - 1u) / per_block);
+    const uint32_t blocks = (uint32_t)(items < cap ? items : cap), rounds = (kept_width + 7u) / 8u;
+    const auto kernel = rounds <= 1u ? page_keep_kernel<1> : rounds <= 2u ? page_keep_kernel<2> : rounds <= 4u ? page_keep_kernel<4> : page_keep_kernel<8>;
+    return (int)launch(kernel, 1u, blocks, kKeepThreads, 0u, stream, p, base, kept, kept_width, per_block);
 }
 
 uint64_t page_workspace_bytes(uint32_t batch, uint32_t width) { return page_ws_bytes(batch, width); }
