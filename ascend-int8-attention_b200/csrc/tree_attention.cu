@@ -1163,41 +1163,55 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const __grid_
     grid_dependency_wait();
     const uint2 *cuts = reinterpret_cast<const uint2 *>(p.at(p.s.cuts));
     const uint32_t i = blockIdx.x + 1u, octet = blockIdx.y;
-    const uint2 cut = __ldcg(cuts + i);
-    if (cut.y == 0 || cut.x >= p.s.slots) return;
-    const uint2 before = __ldcg(cuts + i - 1u);
-    if (before.x == cut.x && before.y != 0) return;           // an earlier cut has the group
-    const Group g = p.groups()[cut.x];
-    if (octet >= (uint32_t)g.octets) return;
-    uint32_t pieces = 2;
-    while (i + pieces - 1u < p.grid) {
-        const uint2 next = __ldcg(cuts + i + pieces - 1u);
-        if (next.x != cut.x || next.y == 0) break;
-        ++pieces;
-    }
+    const uint2 before = __ldcg(cuts + i - 1u), cut = __ldcg(cuts + i), after = __ldcg(cuts + i + 1u);
+    // nothing to join, or an earlier cut has the group
+    if (cut.y == 0 || cut.x >= p.s.slots || (before.x == cut.x && before.y != 0)) return;
     const float *partials = reinterpret_cast<const float *>(p.at(p.s.partials));
     const uint32_t row = octet * kOctet + (threadIdx.x >> 5), lane = threadIdx.x & 31u;
     auto piece = [&](uint32_t q) { return partials + (uint64_t)(q == 0 ? 2u * (i - 1u) + 1u : 2u * (i - 1u + q)) * kPartial; };
+    // The first two pieces, which most groups have no more of, are requested before the group is known: where
+    // they lie depends on the cut alone (rows the group does not have are read in vain).
+    constexpr uint32_t kSums = kGroupRows * kDim, kRefs = kSums + kGroupRows;
+    float4 v[2][4];
+    float refs[2], sums[2];
+#pragma unroll
+    for (uint32_t q = 0; q < 2; ++q) {
+        refs[q] = __ldcg(piece(q) + kRefs + row);
+        sums[q] = __ldcg(piece(q) + kSums + row);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[q][k] = __ldcg(reinterpret_cast<const float4 *>(piece(q) + row * kDim) + k * 32 + lane);
+    }
+    const Group g = p.groups()[cut.x];
+    if (octet >= (uint32_t)g.octets) return;
+    uint32_t pieces = 2;
+    for (uint2 next = after; i + pieces - 1u < p.grid && next.x == cut.x && next.y != 0; next = __ldcg(cuts + i + pieces - 1u)) ++pieces;
     const uint64_t global_row = (uint64_t)g.first_octet * kOctet + row;
     const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + global_row % p.a.heads), sink2 = sink * kLog2e;
-    float at = sink2;
+    float at = fmaxf(sink2, fmaxf(refs[0], refs[1]));
 #pragma unroll 4
-    for (uint32_t q = 0; q < pieces; ++q) at = fmaxf(at, __ldcg(piece(q) + kGroupRows * kDim + kGroupRows + row));
+    for (uint32_t q = 2; q < pieces; ++q) at = fmaxf(at, __ldcg(piece(q) + kRefs + row));
     float total = sink == -INFINITY ? 0.f : kWeightSteps * exp2_approx(sink2 - at);
     float acc[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) acc[k] = 0.f;
-#pragma unroll 2
-    for (uint32_t q = 0; q < pieces; ++q) {
-        const float *src = piece(q);
-        const float f = exp2_approx(__ldcg(src + kGroupRows * kDim + kGroupRows + row) - at);
-        total = fmaf(__ldcg(src + kGroupRows * kDim + row), f, total);
+    auto join = [&](float ref, float sum, const float4 (&o)[4]) {
+        const float f = exp2_approx(ref - at);
+        total = fmaf(sum, f, total);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(src + row * kDim) + k * 32 + lane);
-            acc[4 * k] = fmaf(v.x, f, acc[4 * k]); acc[4 * k + 1] = fmaf(v.y, f, acc[4 * k + 1]);
-            acc[4 * k + 2] = fmaf(v.z, f, acc[4 * k + 2]); acc[4 * k + 3] = fmaf(v.w, f, acc[4 * k + 3]);
+            acc[4 * k] = fmaf(o[k].x, f, acc[4 * k]); acc[4 * k + 1] = fmaf(o[k].y, f, acc[4 * k + 1]);
+            acc[4 * k + 2] = fmaf(o[k].z, f, acc[4 * k + 2]); acc[4 * k + 3] = fmaf(o[k].w, f, acc[4 * k + 3]);
         }
+    };
+    join(refs[0], sums[0], v[0]);
+    join(refs[1], sums[1], v[1]);
+#pragma unroll 2
+    for (uint32_t q = 2; q < pieces; ++q) {
+        const float *src = piece(q);
+        float4 o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = __ldcg(reinterpret_cast<const float4 *>(src + row * kDim) + k * 32 + lane);
+        join(__ldcg(src + kRefs + row), __ldcg(src + kSums + row), o);
     }
     const float inverse = total == 0.f ? 0.f : 1.f / total;
     __nv_bfloat162 *out = reinterpret_cast<__nv_bfloat162 *>(reinterpret_cast<__nv_bfloat16 *>(p.a.out) + global_row * kDim);
@@ -1320,9 +1334,16 @@ int tree_attention(const TreeAttentionArgs *args, cudaStream_t stream)
 {
     if (args == nullptr) return SHAREDKV_EINVAL;
     TreeAttentionArgs a = *args;
-    if (a.tokens == 0 || a.batch == 0) return SHAREDKV_OK;
+    if (a.tokens == 0) return SHAREDKV_OK;
     if (a.ratio != 1u && a.ratio != 4u && a.ratio != 128u) return SHAREDKV_EINVAL;
     if (a.heads == 0 || a.heads % kOctet || a.heads > 128u || a.window == 0 || a.window > 65536u) return SHAREDKV_EINVAL;
+    if (a.batch == 0) {                                       // every row is padding
+        if (!a.out || a.out % 16u || a.lse % 4u) return SHAREDKV_EINVAL;
+        const uint64_t rows = (uint64_t)a.tokens * a.heads;
+        cudaError_t e = cudaMemsetAsync(reinterpret_cast<void *>(a.out), 0, rows * kDim * 2u, stream);
+        if (e == cudaSuccess && a.lse) e = cudaMemsetAsync(reinterpret_cast<void *>(a.lse), 0, rows * 4u, stream);
+        return (int)e;
+    }
     if (a.ratio == 1u) {
         // no compressed kind: its fields alias the original cache so that nothing in the kernel is null
         a.cmp = a.ori; a.cmpScale = a.oriScale; a.cmpTable = a.oriTable; a.cmpStride = a.oriStride;

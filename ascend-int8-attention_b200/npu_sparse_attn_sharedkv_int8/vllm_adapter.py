@@ -23,6 +23,7 @@ import torch
 from .attention import PreparedAttention
 from .cache import PreparedCacheWrite
 from .reference import SharedKVCase
+from .tree_attention import PreparedTreeAttention
 from .runtime import current_stream, native_launcher
 
 SCALE_PROTOCOL = "sharedkv-c8-v1"
@@ -105,6 +106,7 @@ class LayerRuntime:
         self.prefix = impl.swa_cache_layer.prefix.removesuffix(".swa_cache")      # key prefix in the scale file
         self.scales, self.writers = {}, {}                   # kind -> (scale, inverse); geometry -> prepared writer
         self.attention_ops = OrderedDict()                   # geometry -> prepared attention, least recent first
+        self.tree_ops = OrderedDict()                        # the same for drafted trees
         self.captured_ops, self.captured_ids = [], set()     # operators whose launches sit in a captured graph
         self.reported_caches = set()
         self.empty_lse = self.plan = None
@@ -196,6 +198,37 @@ class LayerRuntime:
         result = op.run()
         # outputs belong to the caller (or to the graph's pool); keep only geometry and scratch
         op.case = op.out = op.lse = None
+        if lse is not None:
+            return result, lse.unsqueeze(-1)
+        if self.empty_lse is None:
+            self.empty_lse = torch.empty(0, dtype=torch.float32, device=q.device)
+        return result, self.empty_lse
+
+    def tree_attention(self, q, paths, *, cmp_paths=None, **kw):
+        """Attention of drafted trees (tree_attention.PreparedTreeAttention) with the keyword protocol of
+        `attention`; the query tokens are drafted tokens, `paths` and `cmp_paths` their path masks."""
+        case = self._case_from_call(q, kw)
+        output = torch.empty_like(q)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if kw.get("return_softmax_lse", False) else None
+        shapes = tuple(geometry(v) if isinstance(v, torch.Tensor) else v for v in vars(case).values())
+        # masks are part of the key so that other types or lengths meet the constructor's checks
+        key = (shapes, geometry(paths), geometry(cmp_paths), lse is not None, stream_key(q.device))
+        op = self.tree_ops.get(key)
+        if op is not None:
+            self.tree_ops.move_to_end(key)
+            op._rebind_same_geometry(case, paths, cmp_paths=cmp_paths, output=output, lse_output=lse)
+        else:
+            op = PreparedTreeAttention(case, paths, self.scale("ori", q.device)[0],
+                                       self.scale("cmp", q.device)[0] if case.ratio > 1 else None, cmp_paths=cmp_paths, output=output,
+                                       lse_output=lse, scratch_allocator=scratch_allocator)
+            self.tree_ops[key] = op
+            while len(self.tree_ops) > PREPARED_PER_LAYER:
+                self.tree_ops.popitem(last=False)
+        if torch.cuda.is_current_stream_capturing() and id(op) not in self.captured_ids:
+            self.captured_ids.add(id(op))
+            self.captured_ops.append(op)
+        result = op.run()
+        op.case = op.paths = op.cmp_paths = op.out = op.lse = None
         if lse is not None:
             return result, lse.unsqueeze(-1)
         if self.empty_lse is None:

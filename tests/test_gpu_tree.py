@@ -1,11 +1,13 @@
 """Drafted-tree attention against its definition in float64 (tree_support has the bounds)."""
+from dataclasses import replace
 import math
 import random
+from types import SimpleNamespace
 
 import pytest
 import torch
 
-from npu_sparse_attn_sharedkv_int8 import PreparedAttention, PreparedTreeAttention
+from npu_sparse_attn_sharedkv_int8 import PreparedAttention, PreparedTreeAttention, vllm_adapter
 from npu_sparse_attn_sharedkv_int8.tree_attention import path_masks
 from tests.support import strided_pages
 from tests.tree_support import expected, make_tree_case, signed
@@ -200,11 +202,39 @@ def test_results_do_not_depend_on_the_launch():
         assert torch.equal(op.out, first) and torch.equal(op.lse, lse)
 
 
-def test_no_tokens_and_foreign_shapes():
+def test_no_tokens_and_no_requests():
     made = make_tree_case([2], [10])
     dev, paths, ori_scale, _, _ = on_device(made)
-    dev.q = dev.q[:0]
-    assert PreparedTreeAttention(dev, paths[:0], ori_scale).run().shape == (0, 8, 512)
+    case = replace(dev, q=dev.q[:0])
+    assert PreparedTreeAttention(case, paths[:0], ori_scale).run().shape == (0, 8, 512)
+    case = replace(dev, cu_q=dev.cu_q[:1], seq_lens=dev.seq_lens[:0], ori_block_table=dev.ori_block_table[:0])
+    op = PreparedTreeAttention(case, paths, ori_scale, return_lse=True, output=torch.full_like(dev.q, 7))
+    op.run()
+    assert op.out.eq(0).all() and op.lse.eq(0).all()
+
+
+def test_layer_runtime_route(tmp_path, monkeypatch):
+    """The serving adapter: frozen scales by layer name, operators kept by geometry, other tensors per call."""
+    made = [make_tree_case([6, 9], [700, 130], ratio=128, seed=s) for s in (1, 2)]
+    scales = dict(zip(("model.layers.3.attn.ori", "model.layers.3.attn.cmp"), made[0][3:5]))
+    torch.save({"protocol": "sharedkv-c8-v1", "scales": scales}, tmp_path / "scales.pt")
+    monkeypatch.setenv("SHAREDKV_SCALES", str(tmp_path / "scales.pt"))
+    vllm_adapter.load_scales.cache_clear()
+    impl = SimpleNamespace(head_dim=512, swa_cache_layer=SimpleNamespace(prefix="model.layers.3.attn.swa_cache"))
+    layer = vllm_adapter.runtime(impl)
+    for which in (0, 1, 0):
+        case, paths, cmp_paths = made[which][:3]
+        dev = case.to("cuda")
+        out, lse = layer.tree_attention(
+            dev.q, paths.cuda(), cmp_paths=cmp_paths.cuda(), layout_q="TND", layout_kv="PA_ND", ori_kv=dev.ori, ori_block_table=dev.ori_block_table,
+            cu_seqlens_q=dev.cu_q, seqused_kv=dev.seq_lens, sinks=dev.sink, cmp_kv=dev.cmp, cmp_block_table=dev.cmp_block_table, cmp_ratio=128,
+            ori_win_left=127, softmax_scale=dev.softmax_scale, return_softmax_lse=True)
+        source = (case, paths, cmp_paths, *made[0][3:5])
+        want, want_lse, bound, lse_bound = expected(*source)
+        assert ((out.cpu().double() - want).abs() - bound).max() <= 0
+        assert ((lse[..., 0].cpu().double() - want_lse).abs() - lse_bound).max() <= 0
+    assert len(layer.tree_ops) <= 2
+    vllm_adapter.load_scales.cache_clear()
 
 
 @pytest.mark.parametrize("change, text", [
