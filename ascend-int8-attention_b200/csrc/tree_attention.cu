@@ -51,7 +51,7 @@ constexpr uint32_t kEncodeThreads = 256, kUnionThreads = 1024, kMergeThreads = 2
 constexpr uint32_t kWarpAccumulate = 8, kWarpIssue = 16, kWarpProduce = 18, kProducers = 2;
 // Registers: launched with 96 per thread; accumulate (two warps of every SM partition) grows to hold
 // 128 running sums a thread, the others shrink.
-constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 72, kRegsAccumulate = 152, kRegsIssue = 32;
+constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 64, kRegsAccumulate = 152, kRegsIssue = 48;
 static_assert(2 * kRegsSoftmax + 2 * kRegsAccumulate + kRegsIssue <= 5 * kRegsLaunch, "register shares exceed the launch allocation");
 constexpr float kWeightSteps = 32639.f;                      // 127 * 256 + 127: the largest weight code
 constexpr uint32_t kCodeBias = 0x4b000080u;                  // bits of 2^23 + 128
@@ -62,6 +62,7 @@ constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows 
 constexpr uint32_t kTreeWaitMillions = 4000;                 // cycles, ~2 s: a wait that long is a failure
 // Work split, in tiles: what a group costs besides its tiles, and the shortest piece worth a partial result.
 constexpr uint32_t kGroupCost = 2, kMinPiece = 4;
+constexpr uint32_t kCutSlots = 2048;                         // group slots whose starts the cuts search in shared memory
 
 // shared memory of the walk (dynamic, 1024-byte aligned, all of the 227 KB)
 constexpr uint32_t kSmKey = 0;
@@ -71,8 +72,8 @@ constexpr uint32_t kSmAlpha = kSmWeight + 2 * kSeg;          // FP32 [2 kinds][6
 constexpr uint32_t kSmRef = kSmAlpha + 512;                  // FP32 [64], negated
 constexpr uint32_t kSmTop = kSmRef + 256;                    // INT32 [64] row maxima, as ordered integers
 constexpr uint32_t kSmFactor = kSmTop + 256;                 // FP32 [2][64] rescale factors of a tile
-constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [64] denominators
-constexpr uint32_t kSmInverse = kSmSum + 256;                // FP32 [64]
+constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [3 warps][64] shares of the denominators
+constexpr uint32_t kSmInverse = kSmSum + 768;                // FP32 [64]
 constexpr uint32_t kSmPath = kSmInverse + 256;               // UINT64 [8] paths, UINT64 [8] compressed paths, INT32 [8] path lengths
 constexpr uint32_t kSmFlags = kSmPath + 160;                 // rescale [2 tiles][2 halves], vote [2 halves][3], page masks [4], tmem base, abort
 constexpr uint32_t kSmBars = kSmFlags + 64;
@@ -186,9 +187,9 @@ __device__ __forceinline__ int32_t window_page(int32_t prefix, uint32_t window)
 // kMinPiece tiles (half a range where that is less: with little work, tiles run side by side) moves to the group's edge.  Cut i is (slot, tile): block i walks from cut i to cut i + 1.
 __device__ void cut_tiles(const Tree &p)
 {
-    __shared__ uint32_t sums[33];
+    __shared__ uint32_t sums[33], near[kCutSlots];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x / 32u;
-    uint32_t *starts = reinterpret_cast<uint32_t *>(p.at(p.s.starts));
+    uint32_t *starts = p.s.slots < kCutSlots ? near : reinterpret_cast<uint32_t *>(p.at(p.s.starts));
     const uint32_t per = (p.s.slots + blockDim.x - 1u) / blockDim.x;
     const uint32_t begin = min(threadIdx.x * per, p.s.slots), end = min(begin + per, p.s.slots);
     auto cost = [&](uint32_t slot) {
@@ -439,17 +440,7 @@ __global__ void __launch_bounds__(kUnionThreads, 1) tree_union_kernel(const __gr
             __syncthreads();
             uint32_t before = sums[warp] + incl - sum;
             const uint32_t found = sums[32];
-            for (uint32_t i = begin; i < end; ++i) {
-                base[i] = before;
-                uint32_t bits = bitmap[i];
-                while (bits) {
-                    const uint32_t r = low + i * 32u + (uint32_t)__ffs((int)bits) - 1u;
-                    const int32_t page = table[r / kTreePage];
-                    rows_out[listed + before] = (uint32_t)page < p.a.cmpPages ? (int32_t)((uint32_t)page * kTreePage + (r % kTreePage)) : -1;
-                    ++before;
-                    bits &= bits - 1u;
-                }
-            }
+            for (uint32_t i = begin; i < end; ++i) { base[i] = before; before += __popc(bitmap[i]); }
             for (uint32_t i = threadIdx.x; i < found * 4u; i += kUnionThreads) counts[i] = 0;
             __syncthreads();
 #pragma unroll
@@ -457,6 +448,9 @@ __global__ void __launch_bounds__(kUnionThreads, 1) tree_union_kernel(const __gr
                 const uint32_t r = pick[k] - low;
                 if (pick[k] == 0xffffffffu || pick[k] < low || r >= kUnionRows) continue;
                 const uint32_t rank = base[r / 32u] + __popc(bitmap[r / 32u] & ((1u << (r & 31u)) - 1u));
+                // every thread that names the row writes the same location
+                const int32_t page = table[pick[k] / kTreePage];
+                rows_out[listed + rank] = (uint32_t)page < p.a.cmpPages ? (int32_t)((uint32_t)page * kTreePage + (pick[k] % kTreePage)) : -1;
                 const uint32_t token = first_token + (threadIdx.x + k * kUnionThreads) / p.a.topk;
                 const int32_t o0 = max((int32_t)(token * per_token) - g.first_octet, 0);
                 const int32_t o1 = min((int32_t)((token + 1u) * per_token) - g.first_octet, g.octets);
@@ -567,9 +561,9 @@ struct Items {
 // ------------------------------------------------------------------ walk: producers
 // Two warps take the segments of the tiles in turn: 128 channels of 128 keys, 16 KB.  Pages come as
 // whole boxes of 32 rows x 128 bytes; the listed rows of a ratio-4 layer by gathers of four rows, or
-// row by row when the page stride is no multiple of a row.  Lanes look up pages and rows.  Boxes go out from
-// one elected lane with operands that are the same in the whole warp (51 cycles a box with two warps, 78 when
-// four lanes issue their own); 32 gathers are issued by their lanes.
+// row by row when the page stride is no multiple of a row.  Lanes look up pages and rows; boxes and gathers go
+// out from one elected lane with operands that are the same in the whole warp (with two warps 51 cycles a box
+// and 22 a gather, 78 and 33 when lanes issue their own).
 template <bool LISTED>
 __device__ void produce(const Tree &p, const WalkShared &sm, uint32_t mine, const CUtensorMap *ori_map, const CUtensorMap *cmp_map,
                         const CUtensorMap *row_map, bool gather)
@@ -593,8 +587,8 @@ __device__ void produce(const Tree &p, const WalkShared &sm, uint32_t mine, cons
                     at[i] = row + i < (uint32_t)it.g.cmp_rows ? __ldcg(list + row + i) : -1;
                     found += at[i] >= 0;
                 }
-                there = __ballot_sync(0xffffffffu, found != 0);
-                bytes = gather ? 512u * __popc(there) : 128u * __reduce_add_sync(0xffffffffu, found);
+                there = 0;
+                bytes = gather ? kSeg : 128u * __reduce_add_sync(0xffffffffu, found);
                 if (gather) {
                     const uint32_t per_page = (uint32_t)(p.a.cmpStride / kDim);
 #pragma unroll
@@ -621,10 +615,15 @@ __device__ void produce(const Tree &p, const WalkShared &sm, uint32_t mine, cons
                     mbar_arrive_expect_tx(full, bytes);
                 }
                 if (LISTED && !ori) {
-__syncwarp();
                     if (gather) {
-                        if ((there >> lane) & 1u) tma_gather4(dst + lane * 512u, row_map, (int32_t)(seg * 128u), at[0], at[1], at[2], at[3], full);
+#pragma unroll 8
+                        for (uint32_t g = 0; g < 32u; ++g) {
+                            const int32_t r0 = __shfl_sync(0xffffffffu, at[0], g), r1 = __shfl_sync(0xffffffffu, at[1], g);
+                            const int32_t r2 = __shfl_sync(0xffffffffu, at[2], g), r3 = __shfl_sync(0xffffffffu, at[3], g);
+                            if (leader) tma_gather4(dst + g * 512u, row_map, (int32_t)(seg * 128u), r0, r1, r2, r3, full);
+                        }
                     } else {
+                        __syncwarp();                         // the bytes are announced before any lane asks for some
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (at[i] >= 0)
@@ -658,7 +657,7 @@ __device__ void issue_scores(const Tree &p, const WalkShared &sm, uint32_t tmem)
     constexpr uint32_t kScore = idesc_i8(128, kCodeRows, 0, 0);
     const bool leader = elect_one();
     const uint64_t keys = smem_desc(sm.base + kSmKey, 16u, 1024u, kSwizzle128), query = smem_desc(sm.base + kSmQuery, 16u, 1024u, kSwizzle128);
-    Items<true> it;
+    Items<false> it;
     uint32_t t = 0, sets = 0;
     for (bool more = same(it.first(p)); more; more = same(it.advance(p))) {
         const uint32_t begin = same(it.begin), end = same(it.end), ori_tiles = same((uint32_t)it.g.ori_tiles);
@@ -809,7 +808,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     count = __ldcg(reinterpret_cast<const uint2 *>(p.at(p.s.counts)) + 2u * at + half);
                 sees = (count.x & 0xffffu ? 1u : 0u) | (count.x >> 16 ? 2u : 0u) | (count.y & 0xffffu ? 4u : 0u) | (count.y >> 16 ? 8u : 0u);
             } else {
-                if (!walk_wait<0>(sm, kBarKeyFull + (4u * t) % kRing, ph)) return;      // the page mask comes with segment 0
+                // the page mask comes with segment 0, which the scores have needed
+                if (!walk_wait<0>(sm, kBarScoreFull + buf, ph) || !walk_wait<0>(sm, kBarKeyFull + (4u * t) % kRing, ph)) return;
                 if ((flags[kFlagPages + (t & 3u)] >> warp) & 1u) {
                     const uint64_t *path = reinterpret_cast<const uint64_t *>(sm.ptr + kSmPath) + half * kOctets;
                     if (ori) {
@@ -852,38 +852,39 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 return bias;
             };
             // One octet: integers joined exactly and converted once, log2 weights by packed FMAs, codes, their sums over
-            // the warp, and the codes' bytes to shared memory.  Returns the largest log2 weight.
+            // the warp, and the codes' bytes to shared memory.  True when some weight is above 1.
             uint32_t total = 0;
             auto codes = [&](uint32_t o, const uint32_t *hi, const uint32_t *lo) {
                 const float bias = bias_of(o);
                 const uint64_t bias2 = pack2(bias, bias), steps = pack2(kWeightSteps, kWeightSteps), magic = pack2(8388736.f, 8388736.f);
-                uint32_t d[8], sum[8];
-                float most = -INFINITY;
+                uint32_t pair[4], sum[8], seen_bits = 0;
 #pragma unroll
-                for (uint32_t q = 0; q < 4; ++q) {
-                    const uint64_t a = reinterpret_cast<const uint64_t *>(alpha)[o * 4u + q], off = add2(reinterpret_cast<const uint64_t *>(ref)[o * 4u + q], bias2);
-                    const uint64_t x = fma2(pack2((float)((int32_t)hi[2 * q] * 254 + (int32_t)lo[2 * q]),
-                                                  (float)((int32_t)hi[2 * q + 1] * 254 + (int32_t)lo[2 * q + 1])), a, off);
-                    const float x0 = low2(x), x1 = high2(x);
-                    most = fmaxf(most, fmaxf(x0, x1));
-                    const uint64_t c = fma2(pack2(exp2_approx(x0), exp2_approx(x1)), steps, magic);      // 2^23 + 128 + code
-                    d[2 * q] = __float_as_uint(low2(c));
-                    d[2 * q + 1] = __float_as_uint(high2(c));
+                for (uint32_t q = 0; q < 4; q += 2) {
+                    const ulonglong2 a = reinterpret_cast<const ulonglong2 *>(alpha)[o * 2u + q / 2u], m = reinterpret_cast<const ulonglong2 *>(ref)[o * 2u + q / 2u];
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        const uint32_t r = 2u * (q + e);
+                        const uint64_t x = fma2(pack2((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), (float)((int32_t)hi[r + 1] * 254 + (int32_t)lo[r + 1])),
+                                                e ? a.y : a.x, add2(e ? m.y : m.x, bias2));
+                        const uint64_t c = fma2(pack2(exp2_approx(low2(x)), exp2_approx(high2(x))), steps, magic);      // 2^23 + 128 + code
+                        const uint32_t d0 = (uint32_t)c, d1 = (uint32_t)(c >> 32);
+                        seen_bits |= d0 | d1;
+                        sum[r] = __reduce_add_sync(0xffffffffu, d0);
+                        sum[r + 1] = __reduce_add_sync(0xffffffffu, d1);
+                        pair[q + e] = __byte_perm(d0, d1, 0x5410);
+                    }
                 }
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) sum[i] = __reduce_add_sync(0xffffffffu, d[i]);
                 const uint32_t chunk = half * 2u + (o >> 1), place = (o & 1u) * 8u;
                 *reinterpret_cast<uint2 *>(weights + ((chunk ^ (key & 7u)) << 4) + place) =
-                    make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0051), __byte_perm(d[2], d[3], 0x0051), 0x5410),
-                               __byte_perm(__byte_perm(d[4], d[5], 0x0051), __byte_perm(d[6], d[7], 0x0051), 0x5410));
+                    make_uint2(__byte_perm(pair[0], pair[1], 0x7531), __byte_perm(pair[2], pair[3], 0x7531));
                 *reinterpret_cast<uint2 *>(weights + (((4u + chunk) ^ (key & 7u)) << 4) + place) =
-                    make_uint2(__byte_perm(__byte_perm(d[0], d[1], 0x0040), __byte_perm(d[2], d[3], 0x0040), 0x5410) ^ 0x80808080u,
-                               __byte_perm(__byte_perm(d[4], d[5], 0x0040), __byte_perm(d[6], d[7], 0x0040), 0x5410) ^ 0x80808080u);
+                    make_uint2(__byte_perm(pair[0], pair[1], 0x6420) ^ 0x80808080u, __byte_perm(pair[2], pair[3], 0x6420) ^ 0x80808080u);
                 // lane 8 o + i keeps the sum of row i
                 const uint32_t s01 = lane & 1u ? sum[1] : sum[0], s23 = lane & 1u ? sum[3] : sum[2], s45 = lane & 1u ? sum[5] : sum[4], s67 = lane & 1u ? sum[7] : sum[6];
                 const uint32_t s03 = lane & 2u ? s23 : s01, s47 = lane & 2u ? s67 : s45, s = lane & 4u ? s47 : s03;
                 if ((lane >> 3) == o) total = s - 32u * kCodeBias;
-                return most;
+                // a weight above 1 leaves the 15 bits of a code
+                return (seen_bits & ~(0x4b000000u | 0x7fffu)) != 0;
             };
             // The first tile of an item has no references to start from.
             uint32_t todo = 0xfu;
@@ -895,8 +896,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     tmem_ld16(columns + o * 8u, hi);
                     tmem_ld16(columns + kGroupRows + o * 8u, lo);
                     tmem_wait_ld();
-                    const float first = codes(o, hi, lo), second = codes(o + 1u, hi + 8, lo + 8);
-                    above |= (first > 0.f ? 1u << o : 0u) | (second > 0.f ? 2u << o : 0u);
+                    const bool first = codes(o, hi, lo), second = codes(o + 1u, hi + 8, lo + 8);
+                    above |= (first ? 1u << o : 0u) | (second ? 2u << o : 0u);
                 }
                 if (above) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
                 if (!softmax_sync(sm, half, phase)) return;
@@ -911,19 +912,21 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 // exact row maxima of the octets concerned: integers in float order
                 int32_t high = INT32_MIN;
 #pragma unroll 1
-                for (uint32_t o = 0; o < kOctets; ++o) {
-                    if (!((todo >> o) & 1u)) continue;
-                    uint32_t hi[8], lo[8];
-                    tmem_ld8(columns + o * 8u, hi);
-                    tmem_ld8(columns + kGroupRows + o * 8u, lo);
-                    const float bias = bias_of(o);
+                for (uint32_t o = 0; o < kOctets; o += 2) {
+                    if (!((todo >> o) & 3u)) continue;
+                    uint32_t hi[16], lo[16];
+                    tmem_ld16(columns + o * 8u, hi);
+                    tmem_ld16(columns + kGroupRows + o * 8u, lo);
+                    const float bias[2] = {bias_of(o), bias_of(o + 1u)};
                     tmem_wait_ld();
+                    int32_t v[16];
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i) {
-                        const float x = fmaf((float)((int32_t)hi[i] * 254 + (int32_t)lo[i]), alpha[o * 8u + i], bias);
-                        const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x)));
-                        if (lane == o * 8u + i) high = v;
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        const float x = fmaf((float)((int32_t)hi[i] * 254 + (int32_t)lo[i]), alpha[o * 8u + i], bias[i >> 3]);
+                        v[i] = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x)));
                     }
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) if (lane == o * 8u + i && ((todo >> (o + (i >> 3))) & 1u)) high = v[i];
                 }
                 atomicMax(top + lane, high);
                 if (!softmax_sync(sm, half, phase)) return;
@@ -942,13 +945,14 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 if (!softmax_sync(sm, half, phase)) return;
                 row_sum *= factors[lane];
 #pragma unroll 1
-                for (uint32_t o = 0; o < kOctets; ++o) {
-                    if (!((todo >> o) & 1u)) continue;
-                    uint32_t hi[8], lo[8];
-                    tmem_ld8(columns + o * 8u, hi);
-                    tmem_ld8(columns + kGroupRows + o * 8u, lo);
+                for (uint32_t o = 0; o < kOctets; o += 2) {   // a neighbour that did not move comes out as it was
+                    if (!((todo >> o) & 3u)) continue;
+                    uint32_t hi[16], lo[16];
+                    tmem_ld16(columns + o * 8u, hi);
+                    tmem_ld16(columns + kGroupRows + o * 8u, lo);
                     tmem_wait_ld();
                     codes(o, hi, lo);
+                    codes(o + 1u, hi + 8, lo + 8);
                 }
             }
             tc_fence_before();
@@ -958,16 +962,15 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             row_sum += (float)total;
         }
 
-        // ---- denominators, the warps' shares added in warp order
-#pragma unroll 1
-        for (uint32_t w = 0; w < 4; ++w) {
-            if (warp == w) sums[lane] = w ? sums[lane] + row_sum : row_sum;
-            if (!softmax_sync(sm, half, phase)) return;
-        }
+        // ---- denominators: warp 0 looks after the rows and adds the other warps' shares in warp order
+        if (warp) sums[(warp - 1u) * kGroupRows + lane] = row_sum;
+        if (!softmax_sync(sm, half, phase)) return;
         if (!walk_wait<0>(sm, kBarDoneFree, (items & 1u) ^ 1u)) return;
         if (mine) {
             const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
-            const float a = sm.floats(kSmAlpha)[row0 + key], l = a != a ? a : sums[key], m = -ref[key];      // NaN: a query row that is not finite
+            const float a = sm.floats(kSmAlpha)[row0 + key], m = -ref[key];
+            // a NaN stands for a query row that is not finite
+            const float l = a != a ? a : ((row_sum + sums[key]) + sums[kGroupRows + key]) + sums[2u * kGroupRows + key];
             if (it.whole()) {
                 const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
                 const float sink2 = sink * kLog2e, at = fmaxf(m, sink2), own = exp2_approx(m - at);
