@@ -7,8 +7,7 @@
 // fetched once per group.  A launch is three kernels, four on ratio-4 layers:
 //
 //   tree_encode_kernel   query rows -> two INT8 code planes per cache kind, in the layout of the shared-memory
-//                        operand; group descriptors; rows behind the last live token cleared; its last block
-//                        cuts the launch's tiles into one range per SM
+//                        operand; one block describes the groups and cuts the launch's tiles into a range per SM
 //   tree_union_kernel    (ratio 4) the top-k lists of a group's tokens -> one ascending list of rows with a
 //                        count per token, through a bitmap, so that rows several tokens name are fetched once
 //   tree_walk_kernel     one persistent block per SM: S = K.Q^T and O = K^T.P on the INT8 tensor cores
@@ -61,7 +60,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows a union bitmap covers at a time (32 KB)
 constexpr uint32_t kTreeWaitMillions = 4000;                 // cycles, ~2 s: a wait that long is a failure
 // Work split, in tiles: what a group costs besides its tiles, and the shortest piece worth a partial result.
-constexpr uint32_t kGroupCost = 2, kMinPiece = 4;
+constexpr uint32_t kGroupCost = 2, kMinPiece = 3;
 constexpr uint32_t kCutSlots = 2048;                         // group slots whose starts the cuts search in shared memory
 
 // shared memory of the walk (dynamic, 1024-byte aligned, all of the 227 KB)
@@ -70,11 +69,10 @@ constexpr uint32_t kSmQuery = kSmKey + kRing * kSeg;         // 64 KB: four segm
 constexpr uint32_t kSmWeight = kSmQuery + 4 * kSeg;          // two tiles of weight codes, 128 keys x 128 bytes
 constexpr uint32_t kSmAlpha = kSmWeight + 2 * kSeg;          // FP32 [2 kinds][64]
 constexpr uint32_t kSmRef = kSmAlpha + 512;                  // FP32 [64], negated
-constexpr uint32_t kSmTop = kSmRef + 256;                    // INT32 [64] row maxima, as ordered integers
-constexpr uint32_t kSmFactor = kSmTop + 256;                 // FP32 [2][64] rescale factors of a tile
-constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [3 warps][64] shares of the denominators
-constexpr uint32_t kSmInverse = kSmSum + 768;                // FP32 [64]
-constexpr uint32_t kSmPath = kSmInverse + 256;               // UINT64 [8] paths, UINT64 [8] compressed paths, INT32 [8] path lengths
+constexpr uint32_t kSmTop = kSmRef + 256;                    // INT32 [2][64] row maxima of even and odd tiles, as ordered integers
+constexpr uint32_t kSmFactor = kSmTop + 512;                 // FP32 [2][64] rescale factors of a tile
+constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [3 warps][64] shares of the denominators, then [64] their inverses
+constexpr uint32_t kSmPath = kSmSum + 768;               // UINT64 [8] paths, UINT64 [8] compressed paths, INT32 [8] path lengths
 constexpr uint32_t kSmFlags = kSmPath + 160;                 // rescale [2 tiles][2 halves], vote [2 halves][3], page masks [4], tmem base, abort
 constexpr uint32_t kSmBars = kSmFlags + 64;
 constexpr uint32_t kBarKeyFull = 0, kBarKeyEmpty = 8 /* per two segments */, kBarQueryFull = 12, kBarQueryEmpty = 13, kBarScoreFull = 14,
@@ -92,11 +90,13 @@ struct Group {
 static_assert(sizeof(Group) == 32, "a descriptor is two 16-byte loads");
 
 // ------------------------------------------------------------------ workspace
-// 256 bytes head (word 0 sticky status, word 1 arrivals of the blocks that prepare the walk), cut points,
+// 256 bytes head (word 0 sticky status, word 1 arrivals of the union's blocks, words 2 and 3 the live tokens
+// and the tokens in front of the first request), cut points,
 // group descriptors and starts, query codes and alphas, union lists (ratio 4), partial results.
 struct TreeSpace {
     uint64_t cuts, groups, starts, codes, alphas, rows, counts, partials, bytes;
     uint32_t octets, slots, kinds;
+    uint32_t listed;               // list entries per octet: top-k rounded up to 16-byte loads
 };
 __host__ __device__ inline TreeSpace tree_space(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk)
 {
@@ -111,7 +111,8 @@ __host__ __device__ inline TreeSpace tree_space(uint32_t tokens, uint32_t heads,
     s.codes = up(s.starts + 4ull * (s.slots + 1u));
     s.alphas = up(s.codes + 8192ull * s.kinds * s.octets);
     s.rows = up(s.alphas + 32ull * s.kinds * s.octets);
-    const uint64_t entries = ratio == 4u ? (uint64_t)s.octets * topk : 0ull;
+    s.listed = (topk + 3u) & ~3u;
+    const uint64_t entries = ratio == 4u ? (uint64_t)s.octets * s.listed : 0ull;
     s.counts = up(s.rows + 4ull * entries);
     s.partials = up(s.counts + 16ull * entries);
     s.bytes = s.partials + 2ull * split::kMaxCtas * (kGroupRows * (kDim + 2ull)) * 4ull;
@@ -162,7 +163,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
 // do not run into each other and the slots are in request order; the ones between stay empty.
 __device__ __forceinline__ uint32_t slot_of(uint32_t octets_before, uint32_t request, uint32_t j) { return octets_before / kGroupOctets + request + j; }
 
-// Live requests and tokens (trailing requests without rows or with a negative cumulative count are padding).
+// Live requests (trailing ones without rows or with a negative cumulative count are padding).
 __device__ uint32_t live_requests(const Tree &p, uint32_t *shared)
 {
     if (threadIdx.x == 0) *shared = 0;
@@ -182,9 +183,9 @@ __device__ __forceinline__ int32_t window_page(int32_t prefix, uint32_t window)
 }
 
 // ------------------------------------------------------------------ work split
-// Runs in the last block of the kernel in front of the walk.  The tiles of all groups, each group with
+// Runs in one block of the kernel in front of the walk.  The tiles of all groups, each group with
 // kGroupCost units in front, are cut into p.grid ranges of equal cost; a cut that would leave a piece of fewer than
-// kMinPiece tiles (half a range where that is less: with little work, tiles run side by side) moves to the group's edge.  Cut i is (slot, tile): block i walks from cut i to cut i + 1.
+// kMinPiece tiles (a quarter of a range where that is less: with little work, tiles run side by side) moves to the group's edge.  Cut i is (slot, tile): block i walks from cut i to cut i + 1.
 __device__ void cut_tiles(const Tree &p)
 {
     __shared__ uint32_t sums[33], near[kCutSlots];
@@ -224,7 +225,7 @@ __device__ void cut_tiles(const Tree &p)
     if (threadIdx.x == 0) starts[p.s.slots] = total;
     __syncthreads();
     const uint32_t quota = total ? (total + p.grid - 1u) / p.grid : 1u;
-    const uint32_t shortest = max(1u, min(quota / 2u, kMinPiece));
+    const uint32_t shortest = max(1u, min(quota / 4u, kMinPiece));
     uint2 *cuts = reinterpret_cast<uint2 *>(p.at(p.s.cuts));
     for (uint32_t i = threadIdx.x; i <= p.grid; i += blockDim.x) {
         const uint32_t position = i * quota;
@@ -301,29 +302,16 @@ __device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_
             finite ? alpha * p.a.softmaxScale * (kLog2e / 254.f) : __uint_as_float(0x7fc00000u);
 }
 
-__global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __grid_constant__ Tree p)
+// Group descriptors of all slots, by one block; the head keeps the number of live tokens.
+__device__ void describe_groups(const Tree &p)
 {
     __shared__ uint32_t shared_live;
-    __shared__ __align__(16) float sm_scale[2 * kDim];        // channel 16 l + 4 i + e of a kind at 128 i + 4 l + e
-    grid_dependency_launch_dependents();
-    grid_dependency_wait();
-    const uint32_t lane = threadIdx.x & 31u, row = threadIdx.x >> 5, per_token = p.a.heads / kOctet;
+    const uint32_t per_token = p.a.heads / kOctet;
     const int32_t *cu = p.cu();
-    auto fetch = [&](uint32_t octet, uint4 (&raw)[2]) {
-        const uint4 *src = reinterpret_cast<const uint4 *>(p.a.q + ((uint64_t)octet * kOctet + row) * (kDim * 2u)) + lane * 2u;
-        raw[0] = src[0];
-        raw[1] = src[1];
-    };
-    uint4 raw[2];
-    fetch(blockIdx.x, raw);                                   // in flight while the block finds out what is live
-    for (uint32_t i = threadIdx.x; i < p.s.kinds * kDim; i += kEncodeThreads) {
-        const uint32_t c = i % kDim;
-        sm_scale[i / kDim * kDim + (c >> 2 & 3u) * 128u + (c >> 4) * 4u + (c & 3u)] = __ldg(reinterpret_cast<const float *>(i < kDim ? p.a.oriScale : p.a.cmpScale) + c);
-    }
     const uint32_t live = live_requests(p, &shared_live);
     const uint32_t live_tokens = split::live_token_count(live ? cu[live] : 0, p.a.tokens);
-    // slots of no group: the empty ones between requests, and those behind the last
-    for (uint32_t i = blockIdx.x * kEncodeThreads + threadIdx.x; i < p.s.slots; i += gridDim.x * kEncodeThreads) {
+    if (threadIdx.x == 0) { p.head()[2] = live_tokens; p.head()[3] = live ? min((uint32_t)max(cu[0], 0), live_tokens) : 0u; }
+    for (uint32_t i = threadIdx.x; i < p.s.slots; i += blockDim.x) {
         uint32_t lo = 0, hi = live ? live - 1u : 0u;
         while (lo < hi) {
             const uint32_t mid = (lo + hi + 1u) >> 1;
@@ -352,24 +340,44 @@ __global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __gri
         }
         p.groups()[i] = g;
     }
-    for (uint32_t octet = blockIdx.x; octet < p.s.octets; octet += gridDim.x) {
-        const uint32_t token = octet / per_token;
+    __syncthreads();
+}
+
+// Block 0 plans the walk, the others encode: what is live matters to the plan alone, so the codes of
+// padding rows are computed too (and never read).
+__global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __grid_constant__ Tree p)
+{
+    __shared__ __align__(16) float sm_scale[2 * kDim];        // channel 16 l + 4 i + e of a kind at 128 i + 4 l + e
+    grid_dependency_launch_dependents();
+    grid_dependency_wait();
+    if (blockIdx.x == 0) {
+        describe_groups(p);
+        if (p.a.ratio != 4u) cut_tiles(p);                    // on ratio-4 layers the tiles are known once the lists are joined
+        return;
+    }
+    const uint32_t lane = threadIdx.x & 31u, row = threadIdx.x >> 5, blocks = gridDim.x - 1u;
+    auto fetch = [&](uint32_t octet, uint4 (&raw)[2]) {
+        const uint4 *src = reinterpret_cast<const uint4 *>(p.a.q + ((uint64_t)octet * kOctet + row) * (kDim * 2u)) + lane * 2u;
+        raw[0] = src[0];
+        raw[1] = src[1];
+    };
+    uint32_t octet = blockIdx.x - 1u;
+    uint4 raw[2];
+    fetch(octet, raw);
+    for (uint32_t i = threadIdx.x; i < p.s.kinds * kDim; i += kEncodeThreads) {
+        const uint32_t c = i % kDim;
+        sm_scale[i / kDim * kDim + (c >> 2 & 3u) * 128u + (c >> 4) * 4u + (c & 3u)] = __ldg(reinterpret_cast<const float *>(i < kDim ? p.a.oriScale : p.a.cmpScale) + c);
+    }
+    __syncthreads();
+    for (; octet < p.s.octets; octet += blocks) {
         uint64_t q[8];
         const uint32_t *words = reinterpret_cast<const uint32_t *>(raw);
 #pragma unroll
         for (int i = 0; i < 8; ++i) q[i] = pack2(__uint_as_float(words[i] << 16), __uint_as_float(words[i] & 0xffff0000u));
-        if (octet + gridDim.x < p.s.octets) fetch(octet + gridDim.x, raw);             // the next octet's rows are on their way
-        if (token >= live_tokens || (int32_t)token < cu[0]) {
-            const uint64_t at = ((uint64_t)octet * kOctet + row) * kDim;
-            uint4 *out = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(p.a.out) + at) + lane * 2u;
-            out[0] = out[1] = make_uint4(0, 0, 0, 0);
-            if (p.a.lse && lane == 0) reinterpret_cast<float *>(p.a.lse)[(uint64_t)octet * kOctet + row] = 0.f;
-            continue;
-        }
+        if (octet + blocks < p.s.octets) fetch(octet + blocks, raw);       // the next octet's rows are on their way
 #pragma unroll 1
         for (uint32_t kind = 0; kind < p.s.kinds; ++kind) encode_row(p, kind, octet, row, q, sm_scale);
     }
-    if (p.a.ratio != 4u && last_block(p, gridDim.x)) cut_tiles(p);
 }
 
 // ------------------------------------------------------------------ union of top-k lists
@@ -393,7 +401,7 @@ __global__ void __launch_bounds__(kUnionThreads, 1) tree_union_kernel(const __gr
         const uint32_t limit = (uint32_t)(named < table_rows ? named : table_rows);
         const int32_t *picks = reinterpret_cast<const int32_t *>(p.a.indices) + (uint64_t)first_token * p.a.topk;
         const int32_t *table = reinterpret_cast<const int32_t *>(p.a.cmpTable) + (uint64_t)g.request * p.a.cmpTableWidth;
-        const uint64_t at = (uint64_t)g.first_octet * p.a.topk;
+        const uint64_t at = (uint64_t)g.first_octet * p.s.listed;
         int32_t *rows_out = reinterpret_cast<int32_t *>(p.at(p.s.rows)) + at;
         uint4 *counts_out = reinterpret_cast<uint4 *>(p.at(p.s.counts)) + at;
         uint32_t pick[8];
@@ -450,7 +458,9 @@ __global__ void __launch_bounds__(kUnionThreads, 1) tree_union_kernel(const __gr
                 const uint32_t rank = base[r / 32u] + __popc(bitmap[r / 32u] & ((1u << (r & 31u)) - 1u));
                 // every thread that names the row writes the same location
                 const int32_t page = table[pick[k] / kTreePage];
-                rows_out[listed + rank] = (uint32_t)page < p.a.cmpPages ? (int32_t)((uint32_t)page * kTreePage + (pick[k] % kTreePage)) : -1;
+                const bool there = (uint32_t)page < p.a.cmpPages;
+                rows_out[listed + rank] = there ? (int32_t)((uint32_t)page * kTreePage + (pick[k] % kTreePage)) : -1;
+                if (!there) continue;                         // a missing row counts for nobody
                 const uint32_t token = first_token + (threadIdx.x + k * kUnionThreads) / p.a.topk;
                 const int32_t o0 = max((int32_t)(token * per_token) - g.first_octet, 0);
                 const int32_t o1 = min((int32_t)((token + 1u) * per_token) - g.first_octet, g.octets);
@@ -570,24 +580,40 @@ __device__ void produce(const Tree &p, const WalkShared &sm, uint32_t mine, cons
 {
     const uint32_t lane = threadIdx.x & 31u;
     const bool leader = elect_one();
-    Items<true> it;
+    Items<true> it = {};
     uint32_t tile = 0;                                        // tiles of the block so far: this warp takes segments mine and mine + 2
+    // Looks up tile j: lane l four rows of the list, or for l < 4 the tile's l-th page.
+    int4 raw;
+    auto look = [&](uint32_t j) {
+        raw = make_int4(-1, -1, -1, -1);
+        if (LISTED && j >= (uint32_t)it.g.ori_tiles) {
+            const uint32_t row = (j - (uint32_t)it.g.ori_tiles) * kTile + 4u * lane;
+            if (row < (uint32_t)it.g.cmp_rows)
+                raw = __ldcg(reinterpret_cast<const int4 *>(p.at(p.s.rows) + 4ull * ((uint64_t)it.g.first_octet * p.s.listed + row)));
+        } else {
+            const bool ori = j < (uint32_t)it.g.ori_tiles;
+            const int32_t *table = reinterpret_cast<const int32_t *>(ori ? p.a.oriTable : p.a.cmpTable);
+            const uint32_t width = ori ? p.a.oriTableWidth : p.a.cmpTableWidth;
+            const uint32_t index = (ori ? (uint32_t)window_page(it.g.prefix, p.a.window) + j * 4u : (j - (uint32_t)it.g.ori_tiles) * 4u) + lane;
+            if (lane < 4 && index < width) raw.x = table[(uint64_t)it.g.request * width + index];
+        }
+    };
     for (bool more = it.first(p); more; more = it.advance(p)) {
+        look(it.begin);
         for (uint32_t j = it.begin; j < it.end; ++j, ++tile) {
             const bool ori = j < (uint32_t)it.g.ori_tiles;
-            int32_t at[4] = {-1, -1, -1, -1};
-            uint32_t there, bytes;
+            // what the tile before has looked up for this one
+            int32_t at[4] = {raw.x, raw.y, raw.z, raw.w};
+            if (j + 1u < it.end) look(j + 1u);
+            uint32_t there = 0, bytes;
             if (LISTED && !ori) {
-                // lane l looks up rows 4 l .. 4 l + 3 of the tile
                 const uint32_t row = (j - (uint32_t)it.g.ori_tiles) * kTile + 4u * lane;
-                const int32_t *list = reinterpret_cast<const int32_t *>(p.at(p.s.rows)) + (uint64_t)it.g.first_octet * p.a.topk;
                 uint32_t found = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    at[i] = row + i < (uint32_t)it.g.cmp_rows ? __ldcg(list + row + i) : -1;
+                    if (row + i >= (uint32_t)it.g.cmp_rows) at[i] = -1;
                     found += at[i] >= 0;
                 }
-                there = 0;
                 bytes = gather ? kSeg : 128u * __reduce_add_sync(0xffffffffu, found);
                 if (gather) {
                     const uint32_t per_page = (uint32_t)(p.a.cmpStride / kDim);
@@ -596,11 +622,6 @@ __device__ void produce(const Tree &p, const WalkShared &sm, uint32_t mine, cons
                         at[i] = at[i] < 0 ? 0x7ffffff0 : (int32_t)((uint32_t)at[i] / kTreePage * per_page + (uint32_t)at[i] % kTreePage);
                 }
             } else {
-                // lane l < 4 looks up the tile's l-th page
-                const int32_t *table = reinterpret_cast<const int32_t *>(ori ? p.a.oriTable : p.a.cmpTable);
-                const uint32_t width = ori ? p.a.oriTableWidth : p.a.cmpTableWidth;
-                const uint32_t index = (ori ? (uint32_t)window_page(it.g.prefix, p.a.window) + j * 4u : (j - (uint32_t)it.g.ori_tiles) * 4u) + lane;
-                if (lane < 4 && index < width) at[0] = table[(uint64_t)it.g.request * width + index];
                 there = __ballot_sync(0xffffffffu, (uint32_t)at[0] < (ori ? p.a.oriPages : p.a.cmpPages)) & 15u;
                 bytes = 4096u * __popc(there);
             }
@@ -761,8 +782,6 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
     int32_t *top = reinterpret_cast<int32_t *>(sm.ptr + kSmTop) + half * kRows;
     const uint32_t per_token = p.a.heads / kOctet;
     uint32_t phase = 0, t = 0, vote = kFlagVote + half * 3u;
-    if (key < kRows) top[key] = INT32_MIN;
-
     Items<false> it;
     uint32_t items = 0;
     for (bool more = it.first(p); more; more = it.advance(p), ++items) {
@@ -777,6 +796,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 alpha[key] = mine ? __ldcg(alphas + row) : 0.f;
                 alpha[kGroupRows + key] = mine && p.s.kinds == 2u ? __ldcg(alphas + (uint64_t)p.s.octets * kOctet + row) : 0.f;
                 ref[key] = -kNoKey;
+                top[key] = top[kGroupRows + key] = INT32_MIN;
             } else if (key < kRows + kOctets) {
                 const uint32_t o = half * kOctets + key - kRows;
                 uint64_t m = 0, c = 0;
@@ -793,6 +813,16 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
         }
         if (!softmax_sync(sm, half, phase)) return;
         float row_sum = 0.f;                                  // this warp's share of the denominator of row `lane`
+        float row_ref = kNoKey;                               // reference of row `lane`, the same in every warp of the half
+        const uint32_t present = (1u << max(min(it.g.octets - (int32_t)(half * kOctets), (int32_t)kOctets), 0)) - 1u;
+        const int32_t whole_rows = max(it.g.prefix, 0) / 128;
+        // how often the half's octets name this thread's row of listed tile j
+        auto counts_of = [&](uint32_t j) {
+            const uint32_t entry = (j - (uint32_t)it.g.ori_tiles) * kTile + key;
+            if (entry >= (uint32_t)it.g.cmp_rows) return make_uint2(0, 0);
+            return __ldcg(reinterpret_cast<const uint2 *>(p.at(p.s.counts)) + 2u * ((uint64_t)it.g.first_octet * p.s.listed + entry) + half);
+        };
+        uint2 ahead = make_uint2(0, 0);
 
         for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
             const bool ori = j < (uint32_t)it.g.ori_tiles;
@@ -801,38 +831,31 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             uint32_t sees = 0;
             uint2 count = make_uint2(0x00010001u, 0x00010001u);
             if (LISTED && !ori) {
-                const uint32_t entry = (j - (uint32_t)it.g.ori_tiles) * kTile + key;
-                const uint64_t at = (uint64_t)it.g.first_octet * p.a.topk + entry;
-                count = make_uint2(0, 0);
-                if (entry < (uint32_t)it.g.cmp_rows && __ldcg(reinterpret_cast<const int32_t *>(p.at(p.s.rows)) + at) >= 0)
-                    count = __ldcg(reinterpret_cast<const uint2 *>(p.at(p.s.counts)) + 2u * at + half);
+                count = j == max(it.begin, (uint32_t)it.g.ori_tiles) ? counts_of(j) : ahead;
+                if (j + 1u < it.end) ahead = counts_of(j + 1u);
                 sees = (count.x & 0xffffu ? 1u : 0u) | (count.x >> 16 ? 2u : 0u) | (count.y & 0xffffu ? 4u : 0u) | (count.y >> 16 ? 8u : 0u);
             } else {
-                // the page mask comes with segment 0, which the scores have needed
-                if (!walk_wait<0>(sm, kBarScoreFull + buf, ph) || !walk_wait<0>(sm, kBarKeyFull + (4u * t) % kRing, ph)) return;
-                if ((flags[kFlagPages + (t & 3u)] >> warp) & 1u) {
-                    const uint64_t *path = reinterpret_cast<const uint64_t *>(sm.ptr + kSmPath) + half * kOctets;
-                    if (ori) {
-                        const int32_t *length = reinterpret_cast<const int32_t *>(sm.ptr + kSmPath + 16u * kGroupOctets) + half * kOctets;
-                        const int32_t drafted = window_page(it.g.prefix, p.a.window) * (int32_t)kTreePage + (int32_t)(j * kTile + key) - it.g.prefix;
+                // the page mask came with segment 0, which the scores have needed
+                if (!walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
+                const bool page = (flags[kFlagPages + (t & 3u)] >> warp) & 1u;
+                const int32_t row = (int32_t)((ori ? j : j - (uint32_t)it.g.ori_tiles) * kTile + key);
+                const uint64_t *path = reinterpret_cast<const uint64_t *>(sm.ptr + kSmPath) + half * kOctets;
+                if (ori) {
+                    const int32_t *length = reinterpret_cast<const int32_t *>(sm.ptr + kSmPath + 16u * kGroupOctets) + half * kOctets;
+                    const int32_t drafted = window_page(it.g.prefix, p.a.window) * (int32_t)kTreePage + row - it.g.prefix;
 #pragma unroll
-                        for (uint32_t o = 0; o < kOctets; ++o) {
-                            const bool seen = drafted < 0 ? drafted + (int32_t)p.a.window >= length[o]
-                                                          : drafted < (int32_t)kTreeDraft && ((path[o] >> drafted) & 1ull);
-                            sees |= seen ? 1u << o : 0u;
-                        }
-                    } else {
-                        const int32_t drafted = (int32_t)((j - (uint32_t)it.g.ori_tiles) * kTile + key) - max(it.g.prefix, 0) / 128;
-                        if (drafted < 0) {
-                            sees = 0xfu;
-                        } else if (drafted < (int32_t)kTreeDraft) {
-#pragma unroll
-                            for (uint32_t o = 0; o < kOctets; ++o) sees |= (uint32_t)((path[kGroupOctets + o] >> drafted) & 1ull) << o;
-                        }
+                    for (uint32_t o = 0; o < kOctets; ++o) {
+                        const bool seen = drafted < 0 ? drafted + (int32_t)p.a.window >= length[o]
+                                                      : drafted < (int32_t)kTreeDraft && ((path[o] >> drafted) & 1ull);
+                        sees |= seen ? 1u << o : 0u;
                     }
+                } else if (row < whole_rows) {
+                    sees = 0xfu;
+                } else if (row - whole_rows < (int32_t)kTreeDraft) {
+#pragma unroll
+                    for (uint32_t o = 0; o < kOctets; ++o) sees |= (uint32_t)((path[kGroupOctets + o] >> (row - whole_rows)) & 1ull) << o;
                 }
-                const int32_t present = it.g.octets - (int32_t)(half * kOctets);
-                sees &= (1u << max(min(present, (int32_t)kOctets), 0)) - 1u;
+                sees = page ? sees & present : 0u;
             }
 
             if (!walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
@@ -886,7 +909,23 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 // a weight above 1 leaves the 15 bits of a code
                 return (seen_bits & ~(0x4b000000u | 0x7fffu)) != 0;
             };
-            // The first tile of an item has no references to start from.
+            // Row maxima of octet pair o over this warp's keys, as integers in float order, into `top` (a buffer for even
+            // and one for odd tiles, since a fast warp meets the next tile's maxima while a slow one reads).
+            auto maxima = [&](uint32_t o) {
+                uint32_t hi[16], lo[16];
+                tmem_ld16(columns + o * 8u, hi);
+                tmem_ld16(columns + kGroupRows + o * 8u, lo);
+                const float bias[2] = {bias_of(o), bias_of(o + 1u)};
+                tmem_wait_ld();
+                int32_t high = INT32_MIN;
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) {
+                    const float x = fmaf((float)((int32_t)hi[i] * 254 + (int32_t)lo[i]), alpha[o * 8u + i], bias[i >> 3]);
+                    const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x)));
+                    if (lane == o * 8u + i) high = v;
+                }
+                if (lane >> 4 == o >> 1) atomicMax(top + buf * kGroupRows + lane, high);
+            };
             uint32_t todo = 0xfu;
             if (j != it.begin) {
                 uint32_t above = 0;
@@ -899,51 +938,38 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     const bool first = codes(o, hi, lo), second = codes(o + 1u, hi + 8, lo + 8);
                     above |= (first ? 1u << o : 0u) | (second ? 2u << o : 0u);
                 }
-                if (above) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
+                above = __reduce_or_sync(0xffffffffu, above);
+                if (above) {                                  // only a warp that has such a weight can hold a new maximum
+                    if (lane == 0) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
+#pragma unroll 1
+                    for (uint32_t o = 0; o < kOctets; o += 2) if ((above >> o) & 3u) maxima(o);
+                }
                 if (!softmax_sync(sm, half, phase)) return;
                 todo = flags[vote];
                 const uint32_t zero = kFlagVote + half * 3u;
                 vote = vote == zero + 2u ? zero : vote + 1u;
                 // the word after next was last read before the barrier just passed, and is set behind the next one
                 if (key == 0) flags[vote == zero + 2u ? zero : vote + 1u] = 0;
+            } else {                                          // the first tile of an item has no references to start from
+#pragma unroll 1
+                for (uint32_t o = 0; o < kOctets; o += 2) maxima(o);
+                if (!softmax_sync(sm, half, phase)) return;
             }
             if (key == 0) flags[kFlagRescale + buf * 2u + half] = todo;
             if (todo) {
-                // exact row maxima of the octets concerned: integers in float order
-                int32_t high = INT32_MIN;
-#pragma unroll 1
-                for (uint32_t o = 0; o < kOctets; o += 2) {
-                    if (!((todo >> o) & 3u)) continue;
-                    uint32_t hi[16], lo[16];
-                    tmem_ld16(columns + o * 8u, hi);
-                    tmem_ld16(columns + kGroupRows + o * 8u, lo);
-                    const float bias[2] = {bias_of(o), bias_of(o + 1u)};
-                    tmem_wait_ld();
-                    int32_t v[16];
-#pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) {
-                        const float x = fmaf((float)((int32_t)hi[i] * 254 + (int32_t)lo[i]), alpha[o * 8u + i], bias[i >> 3]);
-                        v[i] = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x)));
-                    }
-#pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) if (lane == o * 8u + i && ((todo >> (o + (i >> 3))) & 1u)) high = v[i];
+                // Every warp works out the new references by itself, from the maxima and the old ones in its
+                // registers, and writes the same values.  Maxima left from earlier tiles lie kHeadroom below
+                // the reference they have led to and move nothing; nor does a NaN.
+                const float highest = __int_as_float(ordered(top[buf * kGroupRows + lane]));
+                float factor = 1.f;
+                if (highest > row_ref - 1.f) {                // the margin covers the rounding of x
+                    factor = exp2_approx(row_ref - (highest + kHeadroom));
+                    row_ref = highest + kHeadroom;
+                    ref[lane] = -row_ref;
                 }
-                atomicMax(top + lane, high);
-                if (!softmax_sync(sm, half, phase)) return;
-                float *factors = sm.floats(kSmFactor) + buf * kGroupRows + row0;
-                if (key < kRows) {
-                    const float highest = __int_as_float(ordered(top[key])), old = -ref[key];
-                    float now = old, factor = 1.f;
-                    if (highest > old - 1.f) {                // the margin covers the rounding of x; a NaN moves nothing
-                        now = highest + kHeadroom;
-                        factor = exp2_approx(old - now);
-                    }
-                    top[key] = INT32_MIN;
-                    ref[key] = -now;
-                    factors[key] = factor;
-                }
-                if (!softmax_sync(sm, half, phase)) return;
-                row_sum *= factors[lane];
+                if (warp == 0) sm.floats(kSmFactor)[buf * kGroupRows + row0 + lane] = factor;
+                row_sum *= factor;
+                __syncwarp();
 #pragma unroll 1
                 for (uint32_t o = 0; o < kOctets; o += 2) {   // a neighbour that did not move comes out as it was
                     if (!((todo >> o) & 3u)) continue;
@@ -963,19 +989,19 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
         }
 
         // ---- denominators: warp 0 looks after the rows and adds the other warps' shares in warp order
+        if (!walk_wait<0>(sm, kBarDoneFree, (items & 1u) ^ 1u)) return;       // the last item's inverses have been read
         if (warp) sums[(warp - 1u) * kGroupRows + lane] = row_sum;
         if (!softmax_sync(sm, half, phase)) return;
-        if (!walk_wait<0>(sm, kBarDoneFree, (items & 1u) ^ 1u)) return;
         if (mine) {
             const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
-            const float a = sm.floats(kSmAlpha)[row0 + key], m = -ref[key];
+            const float a = sm.floats(kSmAlpha)[row0 + key], m = row_ref;
             // a NaN stands for a query row that is not finite
             const float l = a != a ? a : ((row_sum + sums[key]) + sums[kGroupRows + key]) + sums[2u * kGroupRows + key];
             if (it.whole()) {
                 const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
                 const float sink2 = sink * kLog2e, at = fmaxf(m, sink2), own = exp2_approx(m - at);
                 const float all_sum = l * own + (sink == -INFINITY ? 0.f : kWeightSteps * exp2_approx(sink2 - at));
-                sm.floats(kSmInverse)[row0 + key] = all_sum == 0.f ? 0.f : own / all_sum;
+                sm.floats(kSmSum)[row0 + key] = all_sum == 0.f ? 0.f : own / all_sum;
                 if (p.a.lse)
                     reinterpret_cast<float *>(p.a.lse)[row] = all_sum == 0.f ? -INFINITY : (at + log2f(all_sum * (1.f / kWeightSteps))) * kLn2;
             } else {
@@ -997,6 +1023,15 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
 {
     const uint32_t index = threadIdx.x - kWarpAccumulate * 32u, h = index >> 7, channel = index & 127u, warp = channel >> 5;
     const uint32_t tmem_lane = tmem + ((warp * 32u) << 16) + kColOut + h * 32u;
+    {
+        // rows of no live token are cleared
+        const uint32_t live = __ldcg(p.head() + 2) * p.a.heads, skipped = __ldcg(p.head() + 3) * p.a.heads, rows = p.a.tokens * p.a.heads;
+        for (uint32_t i = blockIdx.x; i < skipped + rows - live; i += gridDim.x) {
+            const uint32_t row = i < skipped ? i : live + i - skipped;
+            if (index < 64u) reinterpret_cast<uint4 *>(p.a.out)[(uint64_t)row * 64u + index] = make_uint4(0, 0, 0, 0);
+            if (p.a.lse && index == 64u) reinterpret_cast<float *>(p.a.lse)[row] = 0.f;
+        }
+    }
     Items<false> it;
     uint32_t t = 0, items = 0;
     for (bool more = it.first(p); more; more = it.advance(p), ++items) {
@@ -1068,7 +1103,7 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
         }
         auto value = [&](uint32_t block, uint32_t r) { return r & 1u ? high2(acc[block][r / 2u]) : low2(acc[block][r / 2u]); };
         if (it.whole()) {
-            const float *inverse = sm.floats(kSmInverse) + h * 32u;
+            const float *inverse = sm.floats(kSmSum) + h * 32u;
             __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(p.a.out) + ((uint64_t)it.g.first_octet * kOctet + h * 32u) * kDim + channel;
 #pragma unroll
             for (uint32_t r = 0; r < 32; ++r) {
@@ -1311,8 +1346,8 @@ int tree_launch_all(const TreeAttentionArgs &a, cudaStream_t stream, int sms)
         !tree_map(&row_map, a.cmp, a.cmpStride, a.cmpPages, listed && gather ? 0u : 1u))
         return SHAREDKV_EINVAL;
     static std::atomic<uint64_t> walk_pages{0}, walk_rows{0}, unions{0};
-    const uint32_t encode_blocks = p.s.octets < 4u * (uint32_t)sms ? p.s.octets : 4u * (uint32_t)sms;
-    cudaError_t e = tree_launch(tree_encode_kernel, dim3(encode_blocks), kEncodeThreads, 0u, stream, p);
+    const uint32_t encode_blocks = p.s.octets < 4u * (uint32_t)sms ? p.s.octets : 4u * (uint32_t)sms;      // four fill an SM
+    cudaError_t e = tree_launch(tree_encode_kernel, dim3(encode_blocks + 1u), kEncodeThreads, 0u, stream, p);
     if (e == cudaSuccess && listed) {
         e = tree_opt_in(tree_union_kernel, kUnionSmem, unions);
         if (e == cudaSuccess) e = tree_launch(tree_union_kernel, dim3(p.s.slots), kUnionThreads, kUnionSmem, stream, p);
