@@ -926,11 +926,15 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 }
                 if (lane >> 4 == o >> 1) atomicMax(top + buf * kGroupRows + lane, high);
             };
-            uint32_t todo = 0xfu;
-            if (j != it.begin) {
-                uint32_t above = 0;
+            // Round 0 takes the references as they are (an item's first tile has none and skips it), round 1 redoes the
+            // octets that got new ones.  The code exists once: the warps of this kernel share an instruction cache
+            // that does not hold two copies.
+            uint32_t todo = j == it.begin ? 0u : 0xfu, above = ~todo & 0xfu;
+#pragma unroll 1
+            for (uint32_t round = 0;; ++round) {
 #pragma unroll 1
                 for (uint32_t o = 0; o < kOctets; o += 2) {   // two octets at a time, for loads and arithmetic to overlap
+                    if (!((todo >> o) & 3u)) continue;        // a neighbour that did not move comes out as it was
                     uint32_t hi[16], lo[16];
                     tmem_ld16(columns + o * 8u, hi);
                     tmem_ld16(columns + kGroupRows + o * 8u, lo);
@@ -938,6 +942,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     const bool first = codes(o, hi, lo), second = codes(o + 1u, hi + 8, lo + 8);
                     above |= (first ? 1u << o : 0u) | (second ? 2u << o : 0u);
                 }
+                if (round) break;
                 above = __reduce_or_sync(0xffffffffu, above);
                 if (above) {                                  // only a warp that has such a weight can hold a new maximum
                     if (lane == 0) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
@@ -949,14 +954,11 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 const uint32_t zero = kFlagVote + half * 3u;
                 vote = vote == zero + 2u ? zero : vote + 1u;
                 // the word after next was last read before the barrier just passed, and is set behind the next one
-                if (key == 0) flags[vote == zero + 2u ? zero : vote + 1u] = 0;
-            } else {                                          // the first tile of an item has no references to start from
-#pragma unroll 1
-                for (uint32_t o = 0; o < kOctets; o += 2) maxima(o);
-                if (!softmax_sync(sm, half, phase)) return;
-            }
-            if (key == 0) flags[kFlagRescale + buf * 2u + half] = todo;
-            if (todo) {
+                if (key == 0) {
+                    flags[vote == zero + 2u ? zero : vote + 1u] = 0;
+                    flags[kFlagRescale + buf * 2u + half] = todo;
+                }
+                if (!todo) break;
                 // Every warp works out the new references by itself, from the maxima and the old ones in its
                 // registers, and writes the same values.  Maxima left from earlier tiles lie kHeadroom below
                 // the reference they have led to and move nothing; nor does a NaN.
@@ -970,16 +972,6 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 if (warp == 0) sm.floats(kSmFactor)[buf * kGroupRows + row0 + lane] = factor;
                 row_sum *= factor;
                 __syncwarp();
-#pragma unroll 1
-                for (uint32_t o = 0; o < kOctets; o += 2) {   // a neighbour that did not move comes out as it was
-                    if (!((todo >> o) & 3u)) continue;
-                    uint32_t hi[16], lo[16];
-                    tmem_ld16(columns + o * 8u, hi);
-                    tmem_ld16(columns + kGroupRows + o * 8u, lo);
-                    tmem_wait_ld();
-                    codes(o, hi, lo);
-                    codes(o + 1u, hi + 8, lo + 8);
-                }
             }
             tc_fence_before();
             mbar_arrive(sm.bar(kBarScoreFree + buf));
@@ -1046,8 +1038,8 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
             if (j == (uint32_t)it.g.ori_tiles && j != it.begin) {
 #pragma unroll
                 for (int block = 0; block < 4; ++block) {
-                    const float units = __ldg(reinterpret_cast<const float *>(p.a.oriScale) + block * 128 + channel) /
-                                        __ldg(reinterpret_cast<const float *>(p.a.cmpScale) + block * 128 + channel);
+                    const float units = __fdividef(__ldg(reinterpret_cast<const float *>(p.a.oriScale) + block * 128 + channel),
+                                                   __ldg(reinterpret_cast<const float *>(p.a.cmpScale) + block * 128 + channel));
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[block][r] = mul2(acc[block][r], pack2(units, units));
                 }
