@@ -127,9 +127,16 @@ __device__ void list_free(const Pool &p, uint32_t begin, uint32_t end, uint32_t 
     }
 }
 
-__device__ __forceinline__ void add_ref(const Pool &p, int32_t page, int32_t delta)
+// Adds `delta` to the counts of the pages row[begin .. end - 1] (one warp, four entries of a lane in flight).
+__device__ __forceinline__ void add_refs(const Pool &p, const int32_t *row, uint32_t begin, uint32_t end, int32_t delta, uint32_t lane)
 {
-    if ((uint32_t)page < p.pages) atomicAdd(p.refs + page, delta);
+    for (uint32_t k = begin + lane; k < end; k += 128u) {
+        int32_t page[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) page[i] = k + 32u * i < end ? __ldcg(row + k + 32u * i) : -1;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) if ((uint32_t)page[i] < p.pages) atomicAdd(p.refs + page[i], delta);
+    }
 }
 
 // Finds the `total` lowest free pages; false (for every thread of the cluster) when there are fewer.
@@ -190,7 +197,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_resize_plan(const Pool p
     auto release = [&](int32_t delta) {
         for (uint32_t b = warp; b < p.batch; b += kWarps) {
             const uint32_t before = pages_of(p.lens[b], p.rows), after = pages_of(wanted[b], p.rows);
-            for (uint32_t k = after + lane; k < before; k += 32u) add_ref(p, __ldcg(p.table + (uint64_t)b * p.width + k), delta);
+            add_refs(p, p.table + (uint64_t)b * p.width, after, before, delta, lane);
         }
     };
     release(-1);
@@ -281,8 +288,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
         for (uint32_t b = warp; b < p.batch; b += kWarps) {
             if (children[b] == 1) continue;
             const uint32_t live = pages_of(len[b], p.rows), full = len[b] <= 0 ? 0u : (uint32_t)len[b] / p.rows;
-            for (uint32_t k = lane; k < (children[b] ? full : live); k += 32u)
-                add_ref(p, p.table[(uint64_t)b * p.width + k], sign * (children[b] - 1));
+            add_refs(p, p.table + (uint64_t)b * p.width, 0u, children[b] ? full : live, sign * (children[b] - 1), lane);
         }
     };
     share(1);
@@ -300,9 +306,15 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
     while (columns > 8u && columns * BLOCKS > longest) columns >>= 1;         // a strip for every block, but whole 32-byte sectors
     const uint32_t cells = columns * p.batch, shift = 31u - __clz(columns);
     for (uint32_t left = blockIdx.x * columns; left < longest; left += BLOCKS * columns) {
-        for (uint32_t i = threadIdx.x; i < cells; i += kPlanThreads) {
-            const uint32_t b = i >> shift, k = left + (i & (columns - 1u));
-            if (k < pages_of(len[b], p.rows)) strip[i] = p.table[(uint64_t)b * p.width + k];
+        for (uint32_t base = threadIdx.x; base < cells; base += 8u * kPlanThreads) {
+            int32_t page[8];                                  // eight reads of a thread in flight
+#pragma unroll
+            for (uint32_t n = 0; n < 8; ++n) {
+                const uint32_t i = base + n * kPlanThreads, b = i >> shift, k = left + (i & (columns - 1u));
+                if (i < cells && k < pages_of(len[b], p.rows)) page[n] = p.table[(uint64_t)b * p.width + k];
+            }
+#pragma unroll
+            for (uint32_t n = 0; n < 8; ++n) if (base + n * kPlanThreads < cells) strip[base + n * kPlanThreads] = page[n];
         }
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < cells; i += kPlanThreads) {
