@@ -188,7 +188,7 @@ __device__ __forceinline__ int32_t window_page(int32_t prefix, uint32_t window)
 // kMinPiece tiles (a quarter of a range where that is less: with little work, tiles run side by side) moves to the group's edge.  Cut i is (slot, tile): block i walks from cut i to cut i + 1.
 __device__ void cut_tiles(const Tree &p)
 {
-    __shared__ uint32_t sums[33], near[kCutSlots];
+    __shared__ uint32_t sums[34], near[kCutSlots];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x / 32u;
     uint32_t *starts = p.s.slots < kCutSlots ? near : reinterpret_cast<uint32_t *>(p.at(p.s.starts));
     const uint32_t per = (p.s.slots + blockDim.x - 1u) / blockDim.x;
@@ -198,7 +198,13 @@ __device__ void cut_tiles(const Tree &p)
         return tiles ? tiles + kGroupCost : 0u;
     };
     uint32_t sum = 0;
-    for (uint32_t i = begin; i < end; ++i) sum += cost(i);
+    uint32_t stop = 0;                                        // behind the last group: padding has slots too
+    for (uint32_t i = begin; i < end; ++i) {
+        const uint32_t c = cost(i);
+        sum += c;
+        if (c) stop = i + 1u;
+    }
+    if (threadIdx.x == 0) sums[33] = 0;
     uint32_t incl = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -221,6 +227,7 @@ __device__ void cut_tiles(const Tree &p)
     __syncthreads();
     uint32_t before = sums[warp] + incl - sum;
     for (uint32_t i = begin; i < end; ++i) { starts[i] = before; before += cost(i); }
+    if (stop) atomicMax(sums + 33, stop);
     const uint32_t total = sums[32];
     if (threadIdx.x == 0) starts[p.s.slots] = total;
     __syncthreads();
@@ -229,7 +236,7 @@ __device__ void cut_tiles(const Tree &p)
     uint2 *cuts = reinterpret_cast<uint2 *>(p.at(p.s.cuts));
     for (uint32_t i = threadIdx.x; i <= p.grid; i += blockDim.x) {
         const uint32_t position = i * quota;
-        if (i == p.grid || position >= total) { cuts[i] = make_uint2(p.s.slots, 0); continue; }
+        if (i == p.grid || position >= total) { cuts[i] = make_uint2(sums[33], 0); continue; }
         uint32_t lo = 0, hi = p.s.slots - 1u;                 // last slot that starts at or before the position
         while (lo < hi) {
             const uint32_t mid = (lo + hi + 1u) >> 1;
@@ -911,7 +918,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             };
             // Row maxima of octet pair o over this warp's keys, as integers in float order, into `top` (a buffer for even
             // and one for odd tiles, since a fast warp meets the next tile's maxima while a slow one reads).
-            auto maxima = [&](uint32_t o) {
+            auto maxima = [&](uint32_t o, uint32_t above) {
                 uint32_t hi[16], lo[16];
                 tmem_ld16(columns + o * 8u, hi);
                 tmem_ld16(columns + kGroupRows + o * 8u, lo);
@@ -924,7 +931,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     const int32_t v = __reduce_max_sync(0xffffffffu, ordered(__float_as_int(x)));
                     if (lane == o * 8u + i) high = v;
                 }
-                if (lane >> 4 == o >> 1) atomicMax(top + buf * kGroupRows + lane, high);
+                // rows of an octet that no warp has flagged keep their reference: nothing else of theirs is redone
+                if (lane >> 4 == o >> 1 && ((above >> (lane >> 3)) & 1u)) atomicMax(top + buf * kGroupRows + lane, high);
             };
             // Round 0 takes the references as they are (an item's first tile has none and skips it), round 1 redoes the
             // octets that got new ones.  The code exists once: the warps of this kernel share an instruction cache
@@ -947,7 +955,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 if (above) {                                  // only a warp that has such a weight can hold a new maximum
                     if (lane == 0) atomicOr(const_cast<uint32_t *>(flags) + vote, above);
 #pragma unroll 1
-                    for (uint32_t o = 0; o < kOctets; o += 2) if ((above >> o) & 3u) maxima(o);
+                    for (uint32_t o = 0; o < kOctets; o += 2) if ((above >> o) & 3u) maxima(o, above);
                 }
                 if (!softmax_sync(sm, half, phase)) return;
                 todo = flags[vote];
@@ -987,8 +995,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
         if (mine) {
             const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
             const float a = sm.floats(kSmAlpha)[row0 + key], m = row_ref;
-            // a NaN stands for a query row that is not finite
-            const float l = a != a ? a : ((row_sum + sums[key]) + sums[kGroupRows + key]) + sums[2u * kGroupRows + key];
+            // a NaN stands for a query row that is not finite, as do logits beyond FP32
+            const float l = a != a || m == INFINITY ? __uint_as_float(0x7fc00000u) : ((row_sum + sums[key]) + sums[kGroupRows + key]) + sums[2u * kGroupRows + key];
             if (it.whole()) {
                 const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
                 const float sink2 = sink * kLog2e, at = fmaxf(m, sink2), own = exp2_approx(m - at);

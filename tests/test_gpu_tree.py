@@ -10,7 +10,7 @@ import torch
 from npu_sparse_attn_sharedkv_int8 import PreparedAttention, PreparedTreeAttention, vllm_adapter
 from npu_sparse_attn_sharedkv_int8.tree_attention import path_masks
 from tests.support import strided_pages
-from tests.tree_support import expected, make_tree_case, signed
+from tests.tree_support import check_dense, expected, make_tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -95,6 +95,50 @@ def test_random_geometries(seed):
     check(op, made)
 
 
+LONG = {
+    "c128": dict(counts=[64, 40, 64, 7], prefix=[128 * 2000, 128 * 900 + 77, 128 * 3000 + 5, 128 * 1500], ratio=128),
+    "c128, growing maxima": dict(counts=[64, 64], prefix=[128 * 1800, 128 * 2500], ratio=128, spread=3.0),
+    "c128, 16 heads": dict(counts=[33, 50], prefix=[128 * 1700 + 9, 128 * 800], ratio=128, heads=16, spread=2.0),
+    "c4": dict(counts=[32, 17, 24], prefix=[24000, 9000, 17001], ratio=4, topk=1024),
+    "c4, odd lists": dict(counts=[30, 9], prefix=[14000, 5555], ratio=4, topk=777, spread=2.5),
+    "wide window": dict(counts=[64, 31], prefix=[9000, 5000], window=4000, spread=1.5),
+}
+
+
+@pytest.mark.parametrize("seed", range(3))
+@pytest.mark.parametrize("name", list(LONG))
+def test_many_tiles(name, seed):
+    """Long walks in which references move again and again, on every row."""
+    made = make_tree_case(seed=100 + seed, **LONG[name])
+    dev, paths, ori_scale, cmp_scale, cmp_paths = on_device(made)
+    op = PreparedTreeAttention(dev, paths, ori_scale, cmp_scale, cmp_paths=cmp_paths, return_lse=True)
+    for launch in range(3):
+        op.out.fill_(float("nan"))
+        op.run()
+        worst = check_dense(dev, paths, cmp_paths, ori_scale, cmp_scale, op.out, op.lse)
+        assert worst[0] <= 1 and worst[1] <= 1, (launch, worst)
+    op.status()
+
+
+def test_rising_logits():
+    """Every compressed row scores higher than the one before it: each tile moves every reference."""
+    made = make_tree_case([9, 24], [128 * 700, 128 * 1100], ratio=128, seed=6)
+    case = made[0]
+    direction = (torch.randn(512, generator=torch.Generator().manual_seed(0)) * 20).round().clamp(-60, 60)
+    for b in range(2):
+        pages = case.cmp_block_table[b][case.cmp_block_table[b] >= 0].long()
+        count = pages.numel() * 32
+        slope = torch.linspace(-1, 1, count)[:, None]
+        case.cmp[pages] = (slope * direction + case.cmp[pages].view(count, 512) * 0.2).round().clamp(-127, 127).to(torch.int8).view(-1, 32, 1, 512)
+    case.q = (torch.sign(torch.randn(case.q.shape[:2], generator=torch.Generator().manual_seed(1)))[..., None] * direction / 20
+              + torch.randn(case.q.shape, generator=torch.Generator().manual_seed(2))).to(torch.bfloat16)
+    dev, paths, ori_scale, cmp_scale, cmp_paths = on_device(made)
+    op = PreparedTreeAttention(dev, paths, ori_scale, cmp_scale, cmp_paths=cmp_paths, return_lse=True)
+    op.run()
+    worst = check_dense(dev, paths, cmp_paths, ori_scale, cmp_scale, op.out, op.lse)
+    assert worst[0] <= 1 and worst[1] <= 1, worst
+
+
 @pytest.mark.parametrize("ratio", [1, 4, 128])
 def test_empty_rows_and_sinks(ratio):
     """Paths without a bit, tokens without any key, no sink at all."""
@@ -144,6 +188,22 @@ def test_values_outside_the_keys_do_not_matter():
     keep = torch.ones(got.shape[:2], dtype=torch.bool)
     keep[3, 2] = keep[8, 5] = False
     assert torch.equal(got[keep.cuda()], want[keep.cuda()])
+
+
+def test_logits_beyond_fp32_and_wide_padding():
+    """A query whose logits overflow gives NaN, as the formula does; a batch of capacity 700 with three live
+    requests gives what the three give alone."""
+    made = make_tree_case([4, 9, 2], [300, 90, 128 * 30], ratio=128, seed=21)
+    want = prepared(made).run().clone()
+    case, paths, cmp_paths, ori_scale, cmp_scale = made
+    wide = replace(case, q=case.q.clone(), cu_q=torch.cat([case.cu_q, torch.full((697,), 15, dtype=torch.int32)]),
+                   seq_lens=torch.cat([case.seq_lens, torch.zeros(697, dtype=torch.int32)]),
+                   ori_block_table=torch.cat([case.ori_block_table, torch.zeros(697, case.ori_block_table.shape[1], dtype=torch.int32)]),
+                   cmp_block_table=torch.cat([case.cmp_block_table, torch.zeros(697, case.cmp_block_table.shape[1], dtype=torch.int32)]))
+    assert torch.equal(prepared((wide, paths, cmp_paths, ori_scale, cmp_scale)).run(), want)
+    wide.q[6, 1] = 3e38
+    got = prepared((wide, paths, cmp_paths, ori_scale * 1e6, cmp_scale)).run()
+    assert got[6, 1].isnan().all() and torch.isfinite(got[6, 0]).all()
 
 
 def test_chain_is_the_decode_attention():

@@ -136,3 +136,58 @@ def expected(case, paths, cmp_paths, ori_scale, cmp_scale):
             out_bound[t] = (dw @ v.abs() + out[t].abs() * dw.sum(1, keepdim=True)) / total + out[t].abs() * (BF16_HALF_STEP + 2 ** -20) + 1e-30
             lse_bound[t] = es + (len(v) * ew / total)[:, 0] + lse[t].abs() * 2 ** -20 + 2 ** -20
     return out, lse, out_bound, lse_bound
+
+
+def check_dense(case, paths, cmp_paths, ori_scale, cmp_scale, out, lse):
+    """The bounds above for many keys and tokens, a request at a time on the tensors' device (live requests whose
+    rows all have pages).  Returns the largest errors of out and lse in units of their bounds."""
+    worst = [-math.inf, -math.inf]
+    bits = torch.arange(DRAFT, device=case.q.device)
+    for b in range(case.seq_lens.numel()):
+        first, last = int(case.cu_q[b]), int(case.cu_q[b + 1])
+        n, t = last - first, slice(first, last)
+        prefix = int(case.seq_lens[b]) - n
+        whole = prefix // case.ratio
+
+        def rows(cache, table, logical):
+            return cache[table[b, logical // 32].long(), logical % 32, 0].double()
+
+        start = max(0, prefix - case.window)
+        near = torch.arange(start, prefix + min(n, DRAFT), device=case.q.device)
+        path = ((paths[t, None] >> bits) & 1).bool() & (bits < n)
+        weight = torch.zeros(n, near.numel(), dtype=torch.float64, device=case.q.device)
+        weight[:, :prefix - start] = (near[:prefix - start] >= prefix - (case.window - path.sum(1, keepdim=True))).double()
+        weight[:, prefix - start:] = path[:, :min(n, DRAFT)].double()
+        codes, scales, weights = [rows(case.ori, case.ori_block_table, near)], [ori_scale.double()], [weight]
+        if case.ratio > 1:
+            far = torch.arange(min(whole + DRAFT, case.cmp_block_table.shape[1] * 32), device=case.q.device)
+            weight = torch.zeros(n, whole + DRAFT + 1, dtype=torch.float64, device=case.q.device)
+            if case.ratio == 128:
+                weight[:, :whole] = 1
+                weight[:, whole:whole + DRAFT] = ((cmp_paths[t, None] >> bits) & 1).double()
+            else:
+                picks = case.cmp_indices[t, 0].long()
+                picks = torch.where((picks >= 0) & (picks < whole + DRAFT), picks, whole + DRAFT)
+                weight.scatter_add_(1, picks, torch.ones_like(picks, dtype=torch.float64))
+            codes.append(rows(case.cmp, case.cmp_block_table, far))
+            scales.append(cmp_scale.double())
+            weights.append(weight[:, :far.numel()])
+        v, w0 = torch.cat([c * s for c, s in zip(codes, scales)]), torch.cat(weights, 1)[:, None]
+        q = case.q[t].double()
+        s = torch.einsum("nhd,ld->nhl", q, v) * case.softmax_scale
+        s = s.masked_fill(w0 == 0, -math.inf)
+        sink = case.sink.double()[None, :, None]
+        largest = s.amax(2, keepdim=True)
+        top = torch.maximum(largest, sink)
+        w = (s - top).exp() * w0
+        total = w.sum(2, keepdim=True) + (sink - top).exp()
+        want, want_lse = torch.einsum("nhl,ld->nhd", w, v) / total, (top + total.log())[..., 0]
+        # an entry named k times carries a weight k times as large, and the reference counts from the largest of those
+        lift = (s + w0.clamp_min(1).log()).amax(2, keepdim=True)
+        es = torch.stack([(q * sc).abs().amax(2) * c.abs().sum(1).amax() for c, sc in zip(codes, scales)]).amax(0)[..., None] * case.softmax_scale / 64516
+        dw = w * ((2 * es).exp() - 1) + 4 / 32639 * (lift - top).exp() * (w0 > 0)
+        bound = (torch.einsum("nhl,ld->nhd", dw, v.abs()) + want.abs() * dw.sum(2, keepdim=True)) / total + want.abs() * (BF16_HALF_STEP + 2 ** -20) + 1e-30
+        lse_bound = (es + (w0 > 0).sum(2, keepdim=True) * 4 / 32639 * (lift - top).exp() / total)[..., 0] + want_lse.abs() * 2 ** -20 + 2 ** -20
+        worst[0] = max(worst[0], float(((out[t].double() - want).abs() / bound).max()))
+        worst[1] = max(worst[1], float(((lse[t].double() - want_lse).abs() / lse_bound).max()))
+    return worst
