@@ -2,15 +2,15 @@
 // their page numbering, changed on the device (resize, fork), and the page and row moves that go with
 // them (copy, keep).  The contract is in include/sharedkv_c_abi.h.
 //
-// resize and fork are planned by one cluster of eight thread blocks (one block for small pools), whose
+// resize and fork are planned by one cluster of sixteen thread blocks (one block for small pools), whose
 // hardware barrier separates the phases: the counts of what is released and shared are updated; zeros are counted per warp chunk and the
 // counts added up, which ranks the lowest-numbered free pages; if they do not suffice the count changes are
 // taken back; else they are dealt out in sequence order by a prefix sum.  Counts change by integer
 // atomics, whose sum does not depend on their order; every other value is written by one thread.
-// The plan is a chain of dependent L2 accesses, so it is bound by latency: one block took 126 us for a
-// fork of 512 sequences of 85 pages, most of it one warp after another waiting for table and counts.
-// Pages are copied by a kernel of their own, over all SMs, or by the plan's blocks where that is at
-// most kPlanCopyBytes (always for resize, which copies only shared, partly filled last pages).
+// The plan is a chain of dependent L2 accesses, so it is bound by latency: a fork of 512 sequences of 85 pages
+// with its copies takes 126 us with one block, 28 with eight and 24 with sixteen.
+// Pages are copied by a kernel of their own, over all SMs, or by the plan's blocks where that is at most
+// kPlanCopyBytes (always for resize, which copies only shared, partly filled last pages).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -26,18 +26,18 @@ namespace {
 using ptx::grid_dependency_launch_dependents;
 using ptx::grid_dependency_wait;
 
-constexpr uint32_t kPlanBlocks = 8, kPlanThreads = 1024, kBlockWarps = kPlanThreads / 32;
+constexpr uint32_t kPlanBlocks = 16, kPlanThreads = 1024, kBlockWarps = kPlanThreads / 32;
 constexpr uint32_t kAloneWork = 8192;               // pages + table entries up to which one block is as fast as a cluster
 constexpr uint32_t kMaxSequences = 8192;            // rows whose bookkeeping fits the plan kernel's shared memory
 constexpr uint32_t kStripWords = 16384;             // table entries a fork holds in shared memory at a time
 constexpr uint32_t kCopyThreads = 256;
 constexpr uint64_t kPlanCopyBytes = 1u << 20;        // a second launch costs about what eight blocks need for this much
-constexpr uint32_t kCopyUnit = 8192;                // bytes a thread block moves at a time: two 16-byte loads per thread in flight
+constexpr uint32_t kCopyUnit = 8192, kCopyLoads = kCopyUnit / 16 / kCopyThreads;      // bytes a block moves at a time, 16-byte loads per thread
 constexpr uint32_t kKeepThreads = 256, kMaxKept = 64;
 
 // workspace: word 0 sticky status, word 1 number of page copies, words 64.. chunk counts; then the
 // copy list and the fresh pages
-constexpr uint64_t kWsCounts = 256, kWsCopies = 256 + 4 * 1024;
+constexpr uint64_t kWsCounts = 256, kWsCopies = 256 + 4 * 1024;      // 512 counts fit twice over
 __host__ __device__ constexpr uint64_t page_ws_fresh(uint32_t batch) { return kWsCopies + 8ull * batch; }
 __host__ __device__ constexpr uint64_t page_ws_bytes(uint32_t batch, uint32_t width)
 {
@@ -351,8 +351,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) page_fork_plan(const Pool p, 
     }
 }
 
-// Page copies: unit = 8 KB of one page of one cache; thread blocks walk the units in order.  Streaming:
-// bound by HBM (a page is read and written once), or by latency when there are few.
+// Page copies: unit = 8 KB of one page of one cache; thread blocks walk the units in order.  Streaming: bound by
+// HBM (a page is read and written once; 700 pages in 16 caches move at 5.6 TB/s, 0.86 of a plain copy's rate; twice the
+// unit with half the blocks 5.7, but 3 us more for the 160 pages in 8 caches of a fork), or by latency when there are few.
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const uint64_t *caches, const int2 *pairs, const uint32_t *count_word,
                                                                   uint32_t count, uint32_t layers, uint32_t pages, uint32_t page_bytes)
 {
@@ -371,11 +372,11 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const uint64_t 
         const uint4 *src = reinterpret_cast<const uint4 *>(base + (uint64_t)pair.x * stride + (uint64_t)piece * kCopyUnit);
         uint4 *dst = reinterpret_cast<uint4 *>(base + (uint64_t)pair.y * stride + (uint64_t)piece * kCopyUnit);
         const uint32_t vectors = min(kCopyUnit, page_bytes - piece * kCopyUnit) / 16u;
-        uint4 v[2];
+        uint4 v[kCopyLoads];
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) if (threadIdx.x + i * kCopyThreads < vectors) v[i] = src[threadIdx.x + i * kCopyThreads];
+        for (uint32_t i = 0; i < kCopyLoads; ++i) if (threadIdx.x + i * kCopyThreads < vectors) v[i] = src[threadIdx.x + i * kCopyThreads];
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) if (threadIdx.x + i * kCopyThreads < vectors) dst[threadIdx.x + i * kCopyThreads] = v[i];
+        for (uint32_t i = 0; i < kCopyLoads; ++i) if (threadIdx.x + i * kCopyThreads < vectors) dst[threadIdx.x + i * kCopyThreads] = v[i];
     }
 }
 
@@ -515,15 +516,8 @@ int page_plan(uint32_t op, const PagePoolArgs *args, const int32_t *input, cudaS
     // a fork makes fewer copies than it has sequences
     p.copies_here = (uint64_t)a.batch * a.layers * a.pageRows * 512u <= kPlanCopyBytes;
     cudaError_t e;
-    const bool alone = (uint64_t)a.pages + (uint64_t)a.batch * a.width <= kAloneWork;
-    const uint32_t blocks = alone ? 1u : kPlanBlocks;
-    if (op == 0) {
-        const auto kernel = alone ? page_resize_plan<1> : page_resize_plan<kPlanBlocks>;
-        return (int)launch(kernel, blocks, blocks, kPlanThreads, 4u * a.batch, stream, p, input);
-    }
-    const uint32_t strip = a.batch > kStripWords ? a.batch : kStripWords;
-    const auto kernel = alone ? page_fork_plan<1> : page_fork_plan<kPlanBlocks>;
-    static std::atomic<uint64_t> configured{0};               // opt-in to large dynamic shared memory, per device
+    // Large dynamic shared memory and clusters of more than eight blocks are opted into, once per device.
+    static std::atomic<uint64_t> configured{0};
     int device = 0;
     e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
@@ -532,9 +526,19 @@ int page_plan(uint32_t op, const PagePoolArgs *args, const int32_t *input, cudaS
         constexpr int kMost = (int)(4u * (4u * kMaxSequences + kStripWords));
         e = cudaFuncSetAttribute(page_fork_plan<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(page_fork_plan<kPlanBlocks>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(page_fork_plan<kPlanBlocks>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(page_resize_plan<kPlanBlocks>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return (int)e;
         configured.fetch_or(bit, std::memory_order_relaxed);
     }
+    const bool alone = (uint64_t)a.pages + (uint64_t)a.batch * a.width <= kAloneWork;
+    const uint32_t blocks = alone ? 1u : kPlanBlocks;
+    if (op == 0) {
+        const auto kernel = alone ? page_resize_plan<1> : page_resize_plan<kPlanBlocks>;
+        return (int)launch(kernel, blocks, blocks, kPlanThreads, 4u * a.batch, stream, p, input);
+    }
+    const uint32_t strip = a.batch > kStripWords ? a.batch : kStripWords;
+    const auto kernel = alone ? page_fork_plan<1> : page_fork_plan<kPlanBlocks>;
     e = launch(kernel, blocks, blocks, kPlanThreads, 4u * (4u * a.batch + strip), stream, p, input);
     if (e == cudaSuccess && !p.copies_here) e = launch_copies(a, p.copies, p.head + 1, 0u, a.batch, sms, stream);
     return (int)e;

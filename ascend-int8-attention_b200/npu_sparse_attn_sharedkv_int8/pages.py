@@ -90,8 +90,9 @@ class PagePool:
 
     @staticmethod
     def _check_sequences(tensor, table, name):
-        _require(tensor.dtype == torch.int32 and tuple(tensor.shape) == (table.shape[0],) and tensor.is_contiguous()
-                 and tensor.device == table.device, f"Expected contiguous INT32 {name}[B] on the caches' device")
+        if (tensor.dtype != torch.int32 or tensor.ndim != 1 or tensor.shape[0] != table.shape[0] or not tensor.is_contiguous()
+                or tensor.device != table.device):
+            raise ValueError(f"Expected contiguous INT32 {name}[B] on the caches' device")
 
     def _launch(self, op, first, second=None, count=0):
         index = self.device.index
@@ -129,8 +130,9 @@ class PagePool:
         rows belong to one sequence."""
         _require(self.table is not None, "keep needs a block table")
         self._check_sequences(base, self.table, "base")
-        _require(kept.dtype == torch.int32 and kept.ndim == 2 and kept.shape[0] == self.table.shape[0] and kept.shape[1] <= MAX_KEPT
-                 and kept.is_contiguous() and kept.device == self.device, f"Expected contiguous INT32 kept[B,K <= {MAX_KEPT}] on the caches' device")
+        if (kept.dtype != torch.int32 or kept.ndim != 2 or kept.shape[0] != self.table.shape[0] or kept.shape[1] > MAX_KEPT
+                or not kept.is_contiguous() or kept.device != self.device):
+            raise ValueError(f"Expected contiguous INT32 kept[B,K <= {MAX_KEPT}] on the caches' device")
         if kept.numel():
             self._launch(_KEEP, base, kept, kept.shape[1])
 

@@ -74,7 +74,7 @@ class PreparedTreeAttention:
         _require(cmp_paths is None or case.ratio == 128, "Compressed path masks belong to ratio-128 layers")
         if cmp_paths is not None:
             _check_masks(cmp_paths, tokens, device, "cmp_paths")
-        self.device_index = device.index
+        self.device, self.device_index = device, device.index
         self.scales = (ori_scale, cmp_scale)
         self.kernels = Kernels()
         if self.kernels.lib.sharedkv_tree_args_size() != ctypes.sizeof(_Args):
@@ -128,7 +128,7 @@ class PreparedTreeAttention:
     def status(self):
         """Synchronises the current stream; raises RuntimeError if a wait inside a launch of this operator ran
         out (its results are then invalid).  Diagnostic only."""
-        with torch.cuda.device(self.case.q.device):
+        with torch.cuda.device(self.device):
             check(self.kernels.lib.sharedkv_tree_status(self.args.workspace, current_stream(self.device_index)), "tree attention kernel")
 
 
