@@ -227,6 +227,21 @@ def test_keep(batch, kept, rows, stride):
     check(pool, model)
 
 
+def test_offsets_beyond_32_bits():
+    stride, pages = 1 << 20, 5003
+    cache = torch.empty(pages * stride, dtype=torch.int8, device="cuda").as_strided((pages, 32, 1, 512), (stride, 512, 512, 1))
+    cache[5000:] = torch.randint(-128, 128, (3, 32, 1, 512), dtype=torch.int8, device="cuda")
+    old = cache[5000:].clone()
+    table = ints([[5000, 5001, 5002], [4998, 4999, 0]])
+    pool = PagePool([cache], table)
+    pool.copy(ints([[5001, 4999], [5002, 3]]))
+    pool.keep(ints([40, 0]), ints([[3, 25], [-1, -1]]))                 # rows 43 and 65 of sequence 0 to 40 and 41
+    assert torch.equal(cache[4999], old[1]) and torch.equal(cache[3], old[2])
+    assert torch.equal(cache[5001, 8], old[1, 11]) and torch.equal(cache[5001, 9], old[2, 1])
+    old[1, 8], old[1, 9] = old[1, 11].clone(), old[2, 1].clone()
+    assert torch.equal(cache[5000:], old)
+
+
 def test_captured_steps():
     """A captured grow / fork / trim step, replayed with other inputs."""
     rng = random.Random(77)

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from npu_sparse_attn_sharedkv_int8 import PreparedAttention, PreparedTreeAttention, vllm_adapter
+from npu_sparse_attn_sharedkv_int8.reference import SharedKVCase
 from npu_sparse_attn_sharedkv_int8.tree_attention import path_masks
 from tests.support import strided_pages
 from tests.tree_support import check_dense, expected, make_tree_case
@@ -137,6 +138,88 @@ def test_rising_logits():
     op.run()
     worst = check_dense(dev, paths, cmp_paths, ori_scale, cmp_scale, op.out, op.lse)
     assert worst[0] <= 1 and worst[1] <= 1, worst
+
+
+def test_many_requests():
+    """More group slots than the plan keeps in shared memory."""
+    rng = random.Random(3)
+    counts = [1 + (rng.random() < 0.02) for _ in range(2200)]
+    made = make_tree_case(counts, [rng.randint(0, 40) for _ in counts], seed=8)
+    dev, paths, ori_scale, _, _ = on_device(made)
+    op = PreparedTreeAttention(dev, paths, ori_scale, return_lse=True)
+    op.run()
+    keep = [b for b in range(len(counts)) if b < 40 or b % 97 == 0 or b > 2190]
+    want, want_lse, bound, lse_bound = expected(*made, only=set(keep))
+    rows = torch.tensor([t for b in keep for t in range(int(made[0].cu_q[b]), int(made[0].cu_q[b + 1]))])
+    assert ((op.out.cpu().double() - want).abs() - bound)[rows].max() <= 0
+    assert ((op.lse.cpu().double() - want_lse).abs() - lse_bound)[rows].max() <= 0
+
+
+@pytest.mark.parametrize("ratio", [4, 128])
+def test_contexts_beyond_a_million_rows(ratio):
+    """Lists whose rows pass the span of one bitmap; long tables over a small pool."""
+    gen, rng = torch.Generator().manual_seed(ratio), random.Random(ratio)
+    counts, prefix = [5, 2], [1_300_003, 64]
+    cu = torch.tensor([0, 5, 7], dtype=torch.int32)
+    pool = lambda pages: (torch.randn(pages, 32, 1, 512, generator=gen) * 32).round().clamp(-127, 127).to(torch.int8)  # noqa: E731
+    table = lambda rows, pages: torch.randint(0, pages, (2, -(-rows // 32)), generator=gen, dtype=torch.int32)  # noqa: E731
+    whole = prefix[0] // ratio
+    case = SharedKVCase(q=torch.randn(7, 8, 512, generator=gen).to(torch.bfloat16), ori=pool(40), ori_block_table=table(prefix[0] + 64, 40), cu_q=cu,
+                        seq_lens=torch.tensor([p + n for p, n in zip(prefix, counts)], dtype=torch.int32), sink=torch.linspace(-1, 1, 8), cmp=pool(60),
+                        cmp_block_table=table(whole + 96, 60), ratio=ratio)
+    cmp_paths = None
+    if ratio == 4:
+        case.cmp_indices = torch.full((7, 1, 1024), -1, dtype=torch.int32)
+        for t in range(5):
+            case.cmp_indices[t, 0] = torch.randperm(whole + 64, generator=gen)[:1024].to(torch.int32)
+        case.cmp_indices[5:, 0, :60] = torch.arange(60, dtype=torch.int32)
+    else:
+        cmp_paths = torch.tensor([rng.getrandbits(62) for _ in range(7)])
+    paths = torch.cat([path_masks([-1, 0, 0, 1, 3]), path_masks([-1, -1])])
+    scale = (torch.randn(512, generator=gen) * 0.3).exp() * (4 / 127)
+    dev, paths, ori_scale, cmp_scale, cmp_paths = on_device((case, paths, cmp_paths, scale, scale * 1.1))
+    op = PreparedTreeAttention(dev, paths, ori_scale, cmp_scale, cmp_paths=cmp_paths, return_lse=True)
+    op.run()
+    worst = check_dense(dev, paths, cmp_paths, ori_scale, cmp_scale, op.out, op.lse)
+    assert worst[0] <= 1 and worst[1] <= 1, worst
+
+
+def test_offsets_beyond_32_bits():
+    """Pages more than 4 GB into their cache."""
+    made = make_tree_case([9, 4], [400, 128 * 40], ratio=128, seed=31)
+    dev, paths, ori_scale, cmp_scale, cmp_paths = on_device(made)
+    stride = 1 << 20
+    for name, table in (("ori", "ori_block_table"), ("cmp", "cmp_block_table")):
+        cache, ids = getattr(dev, name), getattr(dev, table)
+        far = 5000 + torch.arange(cache.shape[0], device="cuda", dtype=torch.int32)
+        big = torch.empty((5000 + cache.shape[0]) * stride, dtype=torch.int8, device="cuda").as_strided((5000 + cache.shape[0], 32, 1, 512), (stride, 512, 512, 1))
+        big[5000:] = cache
+        setattr(dev, name, big)
+        setattr(dev, table, torch.where(ids >= 0, far[ids.clamp_min(0).long()], ids))
+    op = PreparedTreeAttention(dev, paths, ori_scale, cmp_scale, cmp_paths=cmp_paths, return_lse=True)
+    op.run()
+    check(op, made)
+
+
+@pytest.mark.parametrize("ratio", [1, 4, 128])
+def test_odd_metadata(ratio):
+    """Tokens in front of the first request, a request without tokens, one with fewer rows than tokens, one
+    without rows at all."""
+    counts, prefix = [3, 0, 5, 4, 6], [200, 50, -3, -4, 77]
+    made = make_tree_case(counts, [max(p, 0) for p in prefix], ratio=ratio, seed=17, topk=20)
+    case = made[0]
+    case.seq_lens = torch.tensor([p + n for p, n in zip(prefix, counts)], dtype=torch.int32)
+    op = prepared(made, return_lse=True)
+    op.run()
+    torch.cuda.synchronize()
+    check(op, made)
+    shifted = replace(case, q=torch.cat([case.q[:3], case.q]), cu_q=case.cu_q + 3)
+    if case.cmp_indices is not None:
+        shifted.cmp_indices = torch.cat([case.cmp_indices[:3], case.cmp_indices])
+    front = lambda t: None if t is None else torch.cat([t[:3], t])  # noqa: E731
+    later = prepared((shifted, front(made[1]), front(made[2]), *made[3:]), return_lse=True)
+    later.run()
+    assert torch.equal(later.out[3:], op.out) and later.out[:3].eq(0).all() and torch.equal(later.lse[3:], op.lse) and later.lse[:3].eq(0).all()
 
 
 @pytest.mark.parametrize("ratio", [1, 4, 128])

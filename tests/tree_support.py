@@ -86,8 +86,8 @@ def make_tree_case(counts, prefix, *, ratio=1, heads=8, window=128, topk=64, see
     return case, torch.tensor([signed(m) for m in masks], dtype=torch.int64), cmp_paths, ori_scale, cmp_scale
 
 
-def expected(case, paths, cmp_paths, ori_scale, cmp_scale):
-    """(out, lse, bound of out, bound of lse) in float64."""
+def expected(case, paths, cmp_paths, ori_scale, cmp_scale, only=None):
+    """(out, lse, bound of out, bound of lse) in float64; of the requests `only` when given."""
     tokens, heads, _ = case.q.shape
     live = max([b + 1 for b in range(case.seq_lens.numel()) if case.seq_lens[b] > 0 and case.cu_q[b + 1] >= 0], default=0)
     out, lse = torch.zeros(tokens, heads, 512, dtype=torch.float64), torch.zeros(tokens, heads, dtype=torch.float64)
@@ -101,6 +101,8 @@ def expected(case, paths, cmp_paths, ori_scale, cmp_scale):
         return cache[index[:, 0], index[:, 1], 0].double()
 
     for b in range(live):
+        if only is not None and b not in only:
+            continue
         first, last = int(case.cu_q[b]), int(case.cu_q[b + 1])
         n = last - first
         prefix = int(case.seq_lens[b]) - n
