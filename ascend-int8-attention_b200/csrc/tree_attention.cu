@@ -873,7 +873,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 sees = page ? sees & present : 0u;
             }
 
-            if (!walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
+            if (LISTED && !walk_wait<0>(sm, kBarScoreFull + buf, ph)) return;
             // the weights of tile t - 2 have been read when its last two key segments have
             if (t >= 2u && !walk_wait<0>(sm, kBarKeyEmpty + 2u * buf + 1u, ph ^ 1u)) return;
             tc_fence_after();

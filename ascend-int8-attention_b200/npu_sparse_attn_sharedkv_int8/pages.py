@@ -75,14 +75,19 @@ class PagePool:
         self.kernels = Kernels()
         if self.kernels.lib.sharedkv_page_args_size() != ctypes.sizeof(_Args):
             raise RuntimeError("Native library ABI changed; rebuild libsharedkv_cuda.so")
-        self._addresses = torch.tensor([[c.data_ptr(), c.stride(0)] for c in caches], dtype=torch.int64).to(device)
         batch, width = (0, 0) if table is None else table.shape
-        # The head of the workspace holds the sticky status; operations write the rest before they read it.
-        # The copy has arrived when it returns, so that the pool may be used on any stream.
-        self.workspace = torch.empty(self.kernels.lib.sharedkv_page_workspace_bytes(batch, width), dtype=torch.uint8, device=device)
-        self.workspace[:256].copy_(torch.zeros(256, dtype=torch.uint8))
+        # One buffer: the caches' addresses and page strides, padded to 256 bytes, then the workspace, whose head
+        # holds the sticky status (operations write the rest before they read it).  The copy has arrived when it
+        # returns, so that the pool may be used on any stream.
+        words = [word for c in caches for word in (c.data_ptr(), c.stride(0))]
+        lead = -(-len(words) // 32) * 32
+        start = torch.tensor(words + [0] * (lead - len(words) + 32), dtype=torch.int64)
+        self._buffer = torch.empty(lead + -(-self.kernels.lib.sharedkv_page_workspace_bytes(batch, width) // 8), dtype=torch.int64, device=device)
+        self._buffer[:lead + 32].copy_(start)
+        self.workspace = self._buffer[lead:]
+        _require(self.workspace.data_ptr() % 256 == 0, "The pool's workspace must be 256-byte aligned")
         self.args = _Args()
-        for name, tensor in (("caches", self._addresses), ("table", table), ("lens", lens), ("refs", refs), ("workspace", self.workspace)):
+        for name, tensor in (("caches", self._buffer), ("table", table), ("lens", lens), ("refs", refs), ("workspace", self.workspace)):
             setattr(self.args, name, 0 if tensor is None else tensor.data_ptr())
         self.args.layers, self.args.pages, self.args.pageRows = len(caches), self.pages, self.page_rows
         self.args.batch, self.args.width = batch, width
