@@ -4,14 +4,14 @@
 // What the tokens of a tree have in common is their keys: eight query rows of 8 heads read the same 512-byte
 // key rows as their neighbours in the tree.  So the unit of work is a GROUP of up to 64 query rows of
 // one request (eight OCTETS; an octet is eight consecutive heads of one token), and a 128-key tile is
-// fetched once per group.  A launch is three kernels, four on ratio-4 layers:
+// fetched once per group.  A launch is two to four kernels:
 //
 //   tree_encode_kernel   query rows -> two INT8 code planes per cache kind, in the layout of the shared-memory
 //                        operand; one block describes the groups and cuts the launch's tiles into a range per SM
 //   tree_union_kernel    (ratio 4) the top-k lists of a group's tokens -> one ascending list of rows with a
 //                        count per token, through a bitmap, so that rows several tokens name are fetched once
 //   tree_walk_kernel     one persistent block per SM: S = K.Q^T and O = K^T.P on the INT8 tensor cores
-//   tree_merge_kernel    joins the partial results of groups that several SMs worked on
+//   tree_merge_kernel    joins the partial results of groups that several SMs worked on  (not for narrow windows)
 //
 // Arithmetic of the walk.  f = q * scale, alpha = max|f| / 127, f ~ alpha (q_hi + q_lo / 254); one MMA
 // of 128 keys x (64 hi rows + 64 lo rows) gives both planes, and the integers are joined exactly,
@@ -61,6 +61,7 @@ constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows 
 constexpr uint32_t kTreeWaitMillions = 4000;                 // cycles, ~2 s: a wait that long is a failure
 // Work split, in tiles: what a group costs besides its tiles, and the shortest piece worth a partial result.
 constexpr uint32_t kGroupCost = 2, kMinPiece = 3;
+constexpr uint32_t kWholeTiles = 3;                          // groups of a window layer that are never split
 constexpr uint32_t kCutSlots = 2048;                         // group slots whose starts the cuts search in shared memory
 
 // shared memory of the walk (dynamic, 1024-byte aligned, all of the 227 KB)
@@ -124,6 +125,7 @@ struct Tree {
     TreeAttentionArgs a;
     TreeSpace s;
     uint32_t grid;                 // blocks of the walk
+    uint32_t splits;               // groups may be worked on by several blocks
     __device__ __forceinline__ char *at(uint64_t offset) const { return reinterpret_cast<char *>(a.workspace) + offset; }
     __device__ __forceinline__ const int32_t *cu() const { return reinterpret_cast<const int32_t *>(a.cuQ); }
     __device__ __forceinline__ const int32_t *seq() const { return reinterpret_cast<const int32_t *>(a.seqLens); }
@@ -237,7 +239,7 @@ __device__ void cut_tiles(const Tree &p)
     if (threadIdx.x == 0) starts[p.s.slots] = total;
     __syncthreads();
     const uint32_t quota = total ? (total + p.grid - 1u) / p.grid : 1u;
-    const uint32_t shortest = max(1u, min(quota / 4u, kMinPiece));
+    const uint32_t shortest = p.splits ? max(1u, min(quota / 4u, kMinPiece)) : 0x40000000u;
     uint2 *cuts = reinterpret_cast<uint2 *>(p.at(p.s.cuts));
     for (uint32_t i = threadIdx.x; i <= p.grid; i += blockDim.x) {
         const uint32_t position = i * quota;
@@ -1353,6 +1355,11 @@ int tree_launch_all(const TreeAttentionArgs &a, cudaStream_t stream, int sms)
     p.a = a;
     p.s = tree_space(a.tokens, a.heads, a.batch, a.ratio, a.topk);
     p.grid = (uint32_t)sms < split::kMaxCtas ? (uint32_t)sms : split::kMaxCtas;
+    // A window layer's groups of two or three tiles stay whole and need no merge kernel: 13.0 against 15.6 us for one
+    // request of 8 tokens (whose two tiles could run side by side), 43.5 against 45.2 us for 48 of 1 to 63 with 16 heads,
+    // 15.3 against 17.0 us for four requests and a window of 200 rows.
+    const uint32_t window_tiles = (a.window + kTreeDraft + kTreePage - 2u) / kTile + 1u;
+    p.splits = a.ratio != 1u || window_tiles > kWholeTiles;
     const bool listed = a.ratio == 4u;
     const bool gather = a.cmpStride % kDim == 0 && (uint64_t)a.cmpPages * (a.cmpStride / kDim) < 0x7ffffff0ull;
     CUtensorMap ori_map, cmp_map, row_map;
@@ -1371,7 +1378,7 @@ int tree_launch_all(const TreeAttentionArgs &a, cudaStream_t stream, int sms)
         e = tree_opt_in(tree_walk_kernel<false>, kWalkSmem, walk_pages);
         if (e == cudaSuccess) e = tree_launch(tree_walk_kernel<false>, dim3(p.grid), kWalkThreads, kWalkSmem, stream, p, ori_map, cmp_map, row_map, 0u);
     }
-    if (e == cudaSuccess && p.grid > 1u) e = tree_launch(tree_merge_kernel, dim3(p.grid - 1u, kGroupOctets), kMergeThreads, 0u, stream, p);
+    if (e == cudaSuccess && p.splits && p.grid > 1u) e = tree_launch(tree_merge_kernel, dim3(p.grid - 1u, kGroupOctets), kMergeThreads, 0u, stream, p);
     return (int)e;
 }
 
