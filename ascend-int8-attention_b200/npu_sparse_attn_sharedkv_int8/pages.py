@@ -92,54 +92,63 @@ class PagePool:
         self.args.layers, self.args.pages, self.args.pageRows = len(caches), self.pages, self.page_rows
         self.args.batch, self.args.width = batch, width
         self.argument_address = ctypes.addressof(self.args)
+        self._page, self._index = self.kernels.lib.sharedkv_page, device.index
 
     @staticmethod
     def _check_sequences(tensor, table, name):
-        if (tensor.dtype != torch.int32 or tensor.ndim != 1 or tensor.shape[0] != table.shape[0] or not tensor.is_contiguous()
-                or tensor.device != table.device):
+        if (tensor.dtype != torch.int32 or tensor.ndim != 1 or len(tensor) != len(table) or not tensor.is_contiguous()
+                or tensor.get_device() != table.get_device()):
             raise ValueError(f"Expected contiguous INT32 {name}[B] on the caches' device")
 
-    def _launch(self, op, first, second=None, count=0):
-        index = self.device.index
-        check(self.kernels.lib.sharedkv_page(self.argument_address, op, first.data_ptr(), 0 if second is None else second.data_ptr(),
-                                             count, index, current_stream(index)), "page pool launch")
+    def _launch(self, op, first, second=0, count=0):
+        index = self._index
+        status = self._page(self.argument_address, op, first, second, count, index, current_stream(index))
+        if status:
+            check(status, "page pool launch")
 
     def resize(self, lens):
         """Sequence b gets lens[b] rows (INT32[B]): more take fresh pages, fewer give pages back, 0 frees
         the sequence.  A growing sequence whose last page is partly filled and shared gets its own copy of
         it.  With too few free pages, or a length the table cannot hold, nothing changes (`status`)."""
-        _require(self.lens is not None, "resize needs lengths and reference counts")
+        if self.lens is None:
+            raise ValueError("resize needs lengths and reference counts")
         self._check_sequences(lens, self.table, "lens")
-        self._launch(_RESIZE, lens)
+        self._launch(_RESIZE, lens.data_ptr())
 
     def fork(self, parents):
         """Sequence b continues sequence parents[b] (INT32[B]; negative: it ends).  The children of a
         sequence share its full pages; the first keeps the partly filled last page, the others get copies.
         With too few free pages or a parent outside the batch nothing changes (`status`)."""
-        _require(self.lens is not None, "fork needs lengths and reference counts")
+        if self.lens is None:
+            raise ValueError("fork needs lengths and reference counts")
         self._check_sequences(parents, self.table, "parents")
-        self._launch(_FORK, parents)
+        self._launch(_FORK, parents.data_ptr())
 
     def copy(self, pairs):
         """Pages pairs[i, 0] -> pairs[i, 1] (INT32[N, 2]) in every cache; pairs outside the pool are
         skipped.  No page may be a destination twice, or a destination and a source."""
-        _require(pairs.dtype == torch.int32 and pairs.ndim == 2 and pairs.shape[1] == 2 and pairs.is_contiguous()
-                 and pairs.device == self.device and pairs.data_ptr() % 8 == 0, "Expected contiguous INT32 pairs[N,2] on the caches' device")
-        if pairs.shape[0]:
-            self._launch(_COPY, pairs, count=pairs.shape[0])
+        address = pairs.data_ptr()
+        if (pairs.dtype != torch.int32 or pairs.ndim != 2 or pairs.shape[1] != 2 or not pairs.is_contiguous()
+                or pairs.get_device() != self._index or address % 8):
+            raise ValueError("Expected contiguous INT32 pairs[N,2] on the caches' device")
+        count = len(pairs)
+        if count:
+            self._launch(_COPY, address, 0, count)
 
     def keep(self, base, kept):
         """Rows base[b] + kept[b, i] -> base[b] + i in every cache (INT32[B], INT32[B, K], K <= 64): packs the
         accepted rows of drafted trees behind the committed ones.  Negative entries and rows without a page
         are skipped; all rows of a sequence are read before one is written.  The pages that hold drafted
         rows belong to one sequence."""
-        _require(self.table is not None, "keep needs a block table")
+        if self.table is None:
+            raise ValueError("keep needs a block table")
         self._check_sequences(base, self.table, "base")
-        if (kept.dtype != torch.int32 or kept.ndim != 2 or kept.shape[0] != self.table.shape[0] or kept.shape[1] > MAX_KEPT
-                or not kept.is_contiguous() or kept.device != self.device):
+        if (kept.dtype != torch.int32 or kept.ndim != 2 or len(kept) != len(self.table) or kept.shape[1] > MAX_KEPT
+                or not kept.is_contiguous() or kept.get_device() != self._index):
             raise ValueError(f"Expected contiguous INT32 kept[B,K <= {MAX_KEPT}] on the caches' device")
-        if kept.numel():
-            self._launch(_KEEP, base, kept, kept.shape[1])
+        width = kept.shape[1]
+        if width and len(kept):
+            self._launch(_KEEP, base.data_ptr(), kept.data_ptr(), width)
 
     def status(self):
         """Synchronises the current stream; raises RuntimeError if a resize or fork of this pool was ever
