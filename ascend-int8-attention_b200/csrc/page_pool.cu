@@ -31,7 +31,7 @@ constexpr uint32_t kAloneWork = 8192;               // pages + table entries up 
 constexpr uint32_t kMaxSequences = 8192;            // rows whose bookkeeping fits the plan kernel's shared memory
 constexpr uint32_t kStripWords = 16384;             // table entries a fork holds in shared memory at a time
 constexpr uint32_t kCopyThreads = 256;
-constexpr uint64_t kPlanCopyBytes = 1u << 20;        // a second launch costs about what eight blocks need for this much
+constexpr uint64_t kPlanCopyBytes = 1u << 20;        // a second launch costs about what the plan's blocks need for this much
 constexpr uint32_t kCopyUnit = 8192, kCopyLoads = kCopyUnit / 16 / kCopyThreads;      // bytes a block moves at a time, 16-byte loads per thread
 constexpr uint32_t kKeepThreads = 256, kMaxKept = 64;
 

@@ -58,6 +58,7 @@ class PagePool:
             _require(shape[0] > 0 and shape[1] > 0 and cache.stride(1) == ROW and cache.stride(-1) == 1
                      and (shape[0] == 1 or cache.stride(0) >= shape[1] * ROW) and shape[1] <= 1 << 20, "Invalid cache strides or empty page storage")
             _require(cache.data_ptr() % 16 == 0 and cache.stride(0) % 16 == 0, "Pages must be 16-byte aligned")
+        _require(len({cache.data_ptr() for cache in caches}) == len(caches), "A cache is in the pool twice")
         _require(lens is None or table is not None, "Lengths need a block table")
         if table is not None:
             _require(table.dtype == torch.int32 and table.ndim == 2 and table.is_contiguous() and table.device == device
@@ -113,7 +114,10 @@ class PagePool:
         if self.lens is None:
             raise ValueError("resize needs lengths and reference counts")
         self._check_sequences(lens, self.table, "lens")
-        self._launch(_RESIZE, lens.data_ptr())
+        address = lens.data_ptr()
+        if address == self.args.lens and address:
+            raise ValueError("The new lens are a tensor of their own: the pool's still say what it holds")
+        self._launch(_RESIZE, address)
 
     def fork(self, parents):
         """Sequence b continues sequence parents[b] (INT32[B]; negative: it ends).  The children of a

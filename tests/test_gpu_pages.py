@@ -295,3 +295,14 @@ def test_refusals():
         PagePool([cache], table).resize(lens)
     with pytest.raises(ValueError, match="block table"):
         PagePool([cache]).keep(lens, table)
+
+
+def test_refuses_aliases():
+    """The pool's own lengths as new ones (a caller who added to them in place would get no pages), and a cache
+    whose rows would move twice."""
+    cache = torch.zeros(8, 32, 1, 512, dtype=torch.int8, device="cuda")
+    table, lens = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="tensor of their own"):
+        PagePool([cache], table, lens).resize(lens)
+    with pytest.raises(ValueError, match="twice"):
+        PagePool([cache, cache], table, lens)
