@@ -20,7 +20,9 @@
 // (15 bits, c_lo signed), so O = 256 O_hi + O_lo is again one exact integer per tile, summed over tiles in
 // FP32 registers; the denominator is the sum of the same codes.  The reference moves only when some
 // logit exceeds it, and then to three powers of two above that logit (kHeadroom): the exact row maximum, a
-// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  The 3 bits this
+// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  A logit is rounded to FP32
+// before the reference is taken off, here as where the maximum is found: a reference at or above all rounded
+// logits leaves no weight above 1, however large they are.  The 3 bits this
 // takes from the codes leave steps of 2^-12 of the largest weight, below a BF16 result's 2^-8.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -54,7 +56,7 @@ constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 64, kRegsAccumulate = 152, k
 static_assert(2 * kRegsSoftmax + 2 * kRegsAccumulate + kRegsIssue <= 5 * kRegsLaunch, "register shares exceed the launch allocation");
 constexpr float kWeightSteps = 32639.f;                      // 127 * 256 + 127: the largest weight code
 constexpr uint32_t kCodeBias = 0x4b000080u;                  // bits of 2^23 + 128
-constexpr float kNoKey = -1e30f;                             // reference of a row that has met no key
+constexpr float kNoKey = -3.402823466e38f;                   // reference of a row that has met no key: the lowest finite value
 constexpr float kHeadroom = 3.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows a union bitmap covers at a time (32 KB)
@@ -904,8 +906,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) {
                         const uint32_t r = 2u * (q + e);
-                        const uint64_t x = fma2(pack2((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), (float)((int32_t)hi[r + 1] * 254 + (int32_t)lo[r + 1])),
-                                                e ? a.y : a.x, add2(e ? m.y : m.x, bias2));
+                        const uint64_t x = add2(fma2(pack2((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), (float)((int32_t)hi[r + 1] * 254 + (int32_t)lo[r + 1])),
+                                                     e ? a.y : a.x, bias2), e ? m.y : m.x);
                         const uint64_t c = fma2(pack2(exp2_approx(low2(x)), exp2_approx(high2(x))), steps, magic);      // 2^23 + 128 + code
                         const uint32_t d0 = (uint32_t)c, d1 = (uint32_t)(c >> 32);
                         seen_bits |= d0 | d1;
@@ -978,11 +980,11 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 }
                 if (!todo) break;
                 // Every warp works out the new references by itself, from the maxima and the old ones in its
-                // registers, and writes the same values.  Maxima left from earlier tiles lie kHeadroom below
+                // registers, and writes the same values.  Maxima left from earlier tiles do not lie above
                 // the reference they have led to and move nothing; nor does a NaN.
                 const float highest = __int_as_float(ordered(top[buf * kGroupRows + lane]));
                 float factor = 1.f;
-                if (highest > row_ref - 1.f) {                // the margin covers the rounding of x
+                if (highest > row_ref) {
                     factor = exp2_approx(row_ref - (highest + kHeadroom));
                     row_ref = highest + kHeadroom;
                     ref[lane] = -row_ref;
