@@ -20,9 +20,9 @@
 // (15 bits, c_lo signed), so O = 256 O_hi + O_lo is again one exact integer per tile, summed over tiles in
 // FP32 registers; the denominator is the sum of the same codes.  The reference moves only when some
 // logit exceeds it, and then to three powers of two above that logit (kHeadroom): the exact row maximum, a
-// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  A logit is rounded to FP32
-// before the reference is taken off, here as where the maximum is found: a reference at or above all rounded
-// logits leaves no weight above 1, however large they are.  The 3 bits this
+// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  Logits are not
+// rounded before the reference is taken off, the maximum is: half a step of FP32, which kHeadroom covers up to 2^20.
+// Beyond, the unit of a row's integers is a power of two, so that its logits have no rounding either.  The 3 bits this
 // takes from the codes leave steps of 2^-12 of the largest weight, below a BF16 result's 2^-8.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -58,6 +58,7 @@ constexpr float kWeightSteps = 32639.f;                      // 127 * 256 + 127:
 constexpr uint32_t kCodeBias = 0x4b000080u;                  // bits of 2^23 + 128
 constexpr float kNoKey = -3.402823466e38f;                   // reference of a row that has met no key: the lowest finite value
 constexpr float kHeadroom = 3.f;
+constexpr float kWideUnit = 0x1p-11f;                        // joined integers stay below 2^31
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows a union bitmap covers at a time (32 KB)
 constexpr uint32_t kTreeWaitMillions = 4000;                 // cycles, ~2 s: a wait that long is a failure
@@ -294,8 +295,15 @@ __device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(high2(f[i]))));
     }
     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));        // as integers a NaN is above all
-    const bool finite = bits < 0x7f800000u;
-    const float alpha = fmaxf(__uint_as_float(bits) * (float)(1.0 / 127), 1e-30f), rcp = __frcp_rn(alpha);
+    const float alpha = fmaxf(__uint_as_float(bits) * (float)(1.0 / 127), 1e-30f);
+    float rcp = __frcp_rn(alpha), unit = alpha * p.a.softmaxScale * (kLog2e / 254.f);          // of the joined integers, as logits to base 2
+    const bool finite = bits < 0x7f800000u && fabsf(unit) < INFINITY;
+    if (fabsf(unit) > kWideUnit) {
+        // logits may pass 2^20: a power of two as unit, up to twice as coarse, makes them exact
+        const float wide = __uint_as_float(min((__float_as_uint(fabsf(unit)) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
+        rcp *= fabsf(unit) / wide;
+        unit = copysignf(wide, unit);
+    }
     // adding 1.5 * 2^23 leaves the nearest integer in the low bits of the sum
     const uint64_t rcp2 = pack2(rcp, rcp), magic = pack2(12582912.f, 12582912.f), minus = pack2(-1.f, -1.f), low = pack2(254.f, 254.f);
     uint32_t hi[4], lo[4];
@@ -317,7 +325,7 @@ __device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_
     *reinterpret_cast<uint4 *>(dst + plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     if (lane == 0)
         reinterpret_cast<float *>(p.at(p.s.alphas))[(uint64_t)(kind * p.s.octets + octet) * kOctet + row] =
-            finite ? alpha * p.a.softmaxScale * (kLog2e / 254.f) : __uint_as_float(0x7fc00000u);
+            finite ? unit : __uint_as_float(0x7fc00000u);
 }
 
 // Group descriptors of all slots, by one block; the head keeps the number of live tokens.
@@ -906,8 +914,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) {
                         const uint32_t r = 2u * (q + e);
-                        const uint64_t x = add2(fma2(pack2((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), (float)((int32_t)hi[r + 1] * 254 + (int32_t)lo[r + 1])),
-                                                     e ? a.y : a.x, bias2), e ? m.y : m.x);
+                        const uint64_t x = fma2(pack2((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), (float)((int32_t)hi[r + 1] * 254 + (int32_t)lo[r + 1])),
+                                                e ? a.y : a.x, add2(e ? m.y : m.x, bias2));
                         const uint64_t c = fma2(pack2(exp2_approx(low2(x)), exp2_approx(high2(x))), steps, magic);      // 2^23 + 128 + code
                         const uint32_t d0 = (uint32_t)c, d1 = (uint32_t)(c >> 32);
                         seen_bits |= d0 | d1;
@@ -984,7 +992,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 // the reference they have led to and move nothing; nor does a NaN.
                 const float highest = __int_as_float(ordered(top[buf * kGroupRows + lane]));
                 float factor = 1.f;
-                if (highest > row_ref) {
+                if (highest > row_ref - 0.5f) {               // the margin covers the rounding of the maximum
                     factor = exp2_approx(row_ref - (highest + kHeadroom));
                     row_ref = highest + kHeadroom;
                     ref[lane] = -row_ref;
