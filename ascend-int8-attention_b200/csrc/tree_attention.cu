@@ -16,14 +16,21 @@
 // Arithmetic of the walk.  f = q * scale, alpha = max|f| / 127, f ~ alpha (q_hi + q_lo / 254); one MMA
 // of 128 keys x (64 hi rows + 64 lo rows) gives both planes, and the integers are joined exactly,
 // S = 254 S_hi + S_lo < 2^31, before the one conversion to FP32.  x = log2(e) s - ref with a reference
-// per row that stays at or above every logit so far; weights 2^x <= 1 become codes c = rint(32639 * 2^x) = 256 c_hi + c_lo
+// per row that stays at or above every logit so far; weights 2^x <= 1 become codes of 32638 steps, c = 256 c_hi + c_lo
 // (15 bits, c_lo signed), so O = 256 O_hi + O_lo is again one exact integer per tile, summed over tiles in
-// FP32 registers; the denominator is the sum of the same codes.  The reference moves only when some
-// logit exceeds it, and then to three powers of two above that logit (kHeadroom): the exact row maximum, a
-// reduction over the 128 lanes that hold the keys, is needed at those tiles alone.  Logits are not
-// rounded before the reference is taken off, the maximum is: half a step of FP32, which kHeadroom covers up to 2^20.
-// Beyond, the unit of a row's integers is a power of two, so that its logits have no rounding either.  The 3 bits this
-// takes from the codes leave steps of 2^-12 of the largest weight, below a BF16 result's 2^-8.
+// FP32 registers.  The codes are the upper bits of 2^23 * 2^x: the denominator sums all 23 bits, exactly per tile, and
+// a number from 0 to 255 that changes from key to key and tile to tile is added before the lower eight are cut off.  So a
+// code errs by less than a step, by none on average, and the errors of n keys add up to some 0.41 sqrt(n) steps; keys
+// that each weigh less than a step are counted as often as their weight asks for.  (Rounded to nearest, and
+// steps of 2^-12, they would all be lost: with one key 10 nats above 8192 others, 10 to 31 % of the output; so it is 0.2 to 0.3 %.)
+// The reference moves only when some logit exceeds it: the exact row maximum, a reduction over the 128 lanes
+// that hold the keys, is needed at those tiles alone.  It then stands three powers of two above the maximum
+// (kHeadroom), and one or two less from the next tile on if the row's weight in this tile is not spread over many keys.  So steps
+// are 2^-14 of the largest weight where one key has most of it, as the decode attention's are, and 2^-12
+// where many keys share it and hide their rounding.  Always one power: 212 us for a C128 batch that takes 176 (every second
+// tile moves references), always three: 174.
+// Logits are not rounded before the reference is taken off, the maximum is: half a step of FP32, which kHeadroom covers up to 2^20.
+// Beyond, the unit of a row's integers is a power of two, so that its logits have no rounding either.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -54,10 +61,11 @@ constexpr uint32_t kWarpAccumulate = 8, kWarpIssue = 16, kWarpProduce = 18, kPro
 // 128 running sums a thread, the others shrink.
 constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 64, kRegsAccumulate = 152, kRegsIssue = 48;
 static_assert(2 * kRegsSoftmax + 2 * kRegsAccumulate + kRegsIssue <= 5 * kRegsLaunch, "register shares exceed the launch allocation");
-constexpr float kWeightSteps = 32639.f;                      // 127 * 256 + 127: the largest weight code
-constexpr uint32_t kCodeBias = 0x4b000080u;                  // bits of 2^23 + 128
+constexpr float kWeightSteps = 32638.f, kFine = 256.f;       // weight 1 in codes (the largest is 127 * 256 + 127), and a code in fine steps
+constexpr uint32_t kCodeBias = 0x4b008000u;                  // bits of 2^23 + 128 * 256
 constexpr float kNoKey = -3.402823466e38f;                   // reference of a row that has met no key: the lowest finite value
-constexpr float kHeadroom = 3.f;
+constexpr float kHeadroom = 3.f;                             // powers of two from a new maximum to the reference
+constexpr uint32_t kSpread = 22;                             // bits of a quarter in fine steps: twice the maximum, seen from the reference
 constexpr float kWideUnit = 0x1p-11f;                        // joined integers stay below 2^31
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows a union bitmap covers at a time (32 KB)
@@ -76,6 +84,7 @@ constexpr uint32_t kSmRef = kSmAlpha + 512;                  // FP32 [64], negat
 constexpr uint32_t kSmTop = kSmRef + 256;                    // INT32 [2][64] row maxima of even and odd tiles, as ordered integers
 constexpr uint32_t kSmFactor = kSmTop + 512;                 // FP32 [2][64] rescale factors of a tile
 constexpr uint32_t kSmSum = kSmFactor + 512;                 // FP32 [3 warps][64] shares of the denominators, then [64] their inverses
+constexpr uint32_t kSmSpread = kSmSum + 256;                 // between tiles of an item, in place of a share: UINT8 [64 rows][4 warps]
 constexpr uint32_t kSmPath = kSmSum + 768;               // UINT64 [8] paths, UINT64 [8] compressed paths, INT32 [8] path lengths
 constexpr uint32_t kSmFlags = kSmPath + 160;                 // rescale [2 tiles][2 halves], vote [2 halves][3], page masks [4], tmem base, abort
 constexpr uint32_t kSmBars = kSmFlags + 64;
@@ -841,6 +850,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
         if (!softmax_sync(sm, half, phase)) return;
         float row_sum = 0.f;                                  // this warp's share of the denominator of row `lane`
         float row_ref = kNoKey;                               // reference of row `lane`, the same in every warp of the half
+        float later = 1.f;                                    // what the row's sums are multiplied by at the next tile
         const uint32_t present = (1u << max(min(it.g.octets - (int32_t)(half * kOctets), (int32_t)kOctets), 0)) - 1u;
         const int32_t whole_rows = max(it.g.prefix, 0) / 128;
         // how often the half's octets name this thread's row of listed tile j
@@ -892,6 +902,10 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             const float *alpha = sm.floats(kSmAlpha) + row0 + (ori ? 0u : kGroupRows);
             char *weights = sm.ptr + kSmWeight + buf * kSeg + key * 128u;
             const uint32_t columns = score + buf * kCodeRows;
+            // What is added to the fine steps of this key's weights before they are cut off: over a warp's keys 32 values 8 apart,
+            // in another order and with another offset in the next warp and tile.  `dithers` is their sum and the codes' bias.
+            const uint32_t dither = (__brev(lane ^ j) >> 24) ^ (2u * warp + (j & 1u));
+            const uint32_t dithers = 32u * (kCodeBias + (dither & 7u)) + 8u * 496u;
             // log2 of how often octet o counts this key: minus infinity where it does not see it
             auto bias_of = [&](uint32_t o) {
                 float bias = (sees >> o) & 1u ? 0.f : -INFINITY;
@@ -906,7 +920,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             uint32_t total = 0;
             auto codes = [&](uint32_t o, const uint32_t *hi, const uint32_t *lo) {
                 const float bias = bias_of(o);
-                const uint64_t bias2 = pack2(bias, bias), steps = pack2(kWeightSteps, kWeightSteps), magic = pack2(8388736.f, 8388736.f);
+                const uint64_t bias2 = pack2(bias, bias), steps = pack2(kWeightSteps * kFine, kWeightSteps * kFine);
+                const uint64_t magic = pack2(__uint_as_float(kCodeBias | dither), __uint_as_float(kCodeBias | dither));
                 uint32_t pair[4], sum[8], seen_bits = 0;
 #pragma unroll
                 for (uint32_t q = 0; q < 4; q += 2) {
@@ -916,12 +931,12 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                         const uint32_t r = 2u * (q + e);
                         const uint64_t x = fma2(pack2((float)((int32_t)hi[r] * 254 + (int32_t)lo[r]), (float)((int32_t)hi[r + 1] * 254 + (int32_t)lo[r + 1])),
                                                 e ? a.y : a.x, add2(e ? m.y : m.x, bias2));
-                        const uint64_t c = fma2(pack2(exp2_approx(low2(x)), exp2_approx(high2(x))), steps, magic);      // 2^23 + 128 + code
+                        const uint64_t c = fma2(pack2(exp2_approx(low2(x)), exp2_approx(high2(x))), steps, magic);      // 2^23 + 256 (128 + code) + fraction + dither
                         const uint32_t d0 = (uint32_t)c, d1 = (uint32_t)(c >> 32);
                         seen_bits |= d0 | d1;
                         sum[r] = __reduce_add_sync(0xffffffffu, d0);
                         sum[r + 1] = __reduce_add_sync(0xffffffffu, d1);
-                        pair[q + e] = __byte_perm(d0, d1, 0x5410);
+                        pair[q + e] = __byte_perm(d0, d1, 0x6521);
                     }
                 }
                 const uint32_t chunk = half * 2u + (o >> 1), place = (o & 1u) * 8u;
@@ -932,9 +947,9 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 // lane 8 o + i keeps the sum of row i
                 const uint32_t s01 = lane & 1u ? sum[1] : sum[0], s23 = lane & 1u ? sum[3] : sum[2], s45 = lane & 1u ? sum[5] : sum[4], s67 = lane & 1u ? sum[7] : sum[6];
                 const uint32_t s03 = lane & 2u ? s23 : s01, s47 = lane & 2u ? s67 : s45, s = lane & 4u ? s47 : s03;
-                if ((lane >> 3) == o) total = s - 32u * kCodeBias;
+                if ((lane >> 3) == o) total = s;
                 // a weight above 1 leaves the 15 bits of a code
-                return (seen_bits & ~(0x4b000000u | 0x7fffu)) != 0;
+                return (seen_bits & ~(0x4b000000u | 0x7fffffu)) != 0;
             };
             // Row maxima of octet pair o over this warp's keys, as integers in float order, into `top` (a buffer for even
             // and one for odd tiles, since a fast warp meets the next tile's maxima while a slow one reads).
@@ -958,6 +973,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             // octets that got new ones.  The code exists once: the warps of this kernel share an instruction cache
             // that does not hold two copies.
             uint32_t todo = j == it.begin ? 0u : 0xfu, above = ~todo & 0xfu;
+            bool moved = false;
 #pragma unroll 1
             for (uint32_t round = 0;; ++round) {
 #pragma unroll 1
@@ -979,33 +995,58 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 }
                 if (!softmax_sync(sm, half, phase)) return;
                 todo = flags[vote];
-                const uint32_t zero = kFlagVote + half * 3u;
+                const uint32_t zero = kFlagVote + half * 3u, low = __ballot_sync(0xffffffffu, later != 1.f);
                 vote = vote == zero + 2u ? zero : vote + 1u;
                 // the word after next was last read before the barrier just passed, and is set behind the next one
                 if (key == 0) {
                     flags[vote == zero + 2u ? zero : vote + 1u] = 0;
-                    flags[kFlagRescale + buf * 2u + half] = todo;
+                    flags[kFlagRescale + buf * 2u + half] = todo | (low & 0xffu ? 1u : 0u) | (low & 0xff00u ? 2u : 0u) | (low & 0xff0000u ? 4u : 0u) | (low >> 24 ? 8u : 0u);
                 }
-                if (!todo) break;
+                float factor = later;
+                later = 1.f;
+                if (!todo) {
+                    if (low && warp == 0) sm.floats(kSmFactor)[buf * kGroupRows + row0 + lane] = factor;
+                    break;
+                }
                 // Every warp works out the new references by itself, from the maxima and the old ones in its
-                // registers, and writes the same values.  Maxima left from earlier tiles do not lie above
-                // the reference they have led to and move nothing; nor does a NaN.
+                // registers, and writes the same values; of the octets that are done again only.  Maxima left from
+                // earlier tiles do not lie above the reference they have led to and move nothing; nor does a NaN.
                 const float highest = __int_as_float(ordered(top[buf * kGroupRows + lane]));
-                float factor = 1.f;
-                if (highest > row_ref - 0.5f) {               // the margin covers the rounding of the maximum
-                    factor = exp2_approx(row_ref - (highest + kHeadroom));
+                if (((todo >> (lane >> 3)) & 1u) && highest > row_ref - 0.5f) {               // the margin covers the rounding of the maximum
+                    const float down = exp2_approx(row_ref - (highest + kHeadroom));
                     row_ref = highest + kHeadroom;
                     ref[lane] = -row_ref;
+                    factor *= down;
+                    row_sum *= down;
+                    moved = true;
                 }
                 if (warp == 0) sm.floats(kSmFactor)[buf * kGroupRows + row0 + lane] = factor;
-                row_sum *= factor;
                 __syncwarp();
             }
             tc_fence_before();
             mbar_arrive(sm.bar(kBarScoreFree + buf));
             fence_proxy_async_smem();
             mbar_arrive(sm.bar(kBarWeightReady + buf));
-            row_sum += (float)total;
+            row_sum = fmaf((float)(total - dithers), 1.f / kFine, row_sum);
+            // Where a new maximum leaves little weight for others, the reference may be close to it from the next tile on:
+            // where the second heaviest of the tile's four runs of 32 keys weighs less than twice the maximum.  Not for the
+            // sake of one last tile (44.3 against 44.8 us on the window batch).
+            if (todo && j + 2u < it.end) {
+                uint8_t *spread = reinterpret_cast<uint8_t *>(sm.ptr + kSmSpread) + (row0 + lane) * 4u;
+                spread[warp] = (uint8_t)(32 - __clz((int32_t)(total - dithers)));
+                if (!softmax_sync(sm, half, phase)) return;
+                const uint32_t bits = *reinterpret_cast<const uint32_t *>(spread);
+                const uint32_t b0 = bits & 255u, b1 = (bits >> 8) & 255u, b2 = (bits >> 16) & 255u, b3 = bits >> 24;
+                const uint32_t second = max(max(min(b0, b1), min(b2, b3)), min(max(b0, b1), max(b2, b3)));
+                if (moved && second < kSpread) {
+                    const float next = row_ref - (float)min(kSpread - second, 2u);
+                    later = exp2_approx(row_ref - next);
+                    row_ref = next;
+                    row_sum *= later;
+                    ref[lane] = -next;
+                }
+                __syncwarp();
+            }
         }
 
         // ---- denominators: warp 0 looks after the rows and adds the other warps' shares in warp order
