@@ -143,16 +143,19 @@ class PagePool:
         """Rows base[b] + kept[b, i] -> base[b] + i in every cache (INT32[B], INT32[B, K], K <= 64): packs the
         accepted rows of drafted trees behind the committed ones.  Negative entries and rows without a page
         are skipped; all rows of a sequence are read before one is written.  The pages that hold drafted
-        rows belong to one sequence."""
+        rows belong to one sequence.  `base` is a tensor of its own: the pool's lens include the draft since the
+        resize that made room for it."""
         if self.table is None:
             raise ValueError("keep needs a block table")
         self._check_sequences(base, self.table, "base")
         if (kept.dtype != torch.int32 or kept.ndim != 2 or len(kept) != len(self.table) or kept.shape[1] > MAX_KEPT
                 or not kept.is_contiguous() or kept.get_device() != self._index):
             raise ValueError(f"Expected contiguous INT32 kept[B,K <= {MAX_KEPT}] on the caches' device")
-        width = kept.shape[1]
+        width, address = kept.shape[1], base.data_ptr()
+        if address == self.args.lens and address:
+            raise ValueError("base is a tensor of its own, the committed lengths: the pool's lens include the draft")
         if width and len(kept):
-            self._launch(_KEEP, base.data_ptr(), kept.data_ptr(), width)
+            self._launch(_KEEP, address, kept.data_ptr(), width)
 
     def status(self):
         """Synchronises the current stream; raises RuntimeError if a resize or fork of this pool was ever

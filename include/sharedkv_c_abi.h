@@ -330,7 +330,8 @@ SHAREDKV_API int launch_page_fork(void *stream, const PagePoolArgs *args, const 
 SHAREDKV_API int launch_page_copy(void *stream, const PagePoolArgs *args, const int32_t *pairs, uint32_t count);
 /* Rows base[b] + kept[b, i] -> base[b] + i (INT32 [batch], [batch, width_kept <= 64], device) in every
  * cache: the accepted rows of a drafted tree move up behind the committed ones.  Negative entries and
- * rows without a page are skipped; all rows of a sequence are read before one is written. */
+ * rows without a page are skipped; all rows of a sequence are read before one is written.  `base` are
+ * the committed lengths, not the pool's `lens`, which a resize has made include the draft. */
 SHAREDKV_API int launch_page_keep(void *stream, const PagePoolArgs *args, const int32_t *base, const int32_t *kept, uint32_t kept_width);
 /* Host-bridge forms: `op` 0 resize, 1 fork, 2 copy, 3 keep; `a`, `b` the device arrays, `n` the count. */
 SHAREDKV_API int sharedkv_page(uint64_t args, uint32_t op, uint64_t a, uint64_t b, uint32_t n, int32_t device, void *stream);
