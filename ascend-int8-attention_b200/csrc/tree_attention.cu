@@ -823,14 +823,21 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
     for (bool more = it.first(p); more; more = it.advance(p), ++items) {
         const uint32_t row0 = half * kRows;                   // first row of the half in the group
         const bool mine = key < kRows && row0 + key < (uint32_t)it.g.octets * kOctet;          // this thread looks after row `key` of the half
+        float row_sum = 0.f;                                  // this warp's share of the denominator of row `lane`
         {
             uint64_t *path = reinterpret_cast<uint64_t *>(sm.ptr + kSmPath);
             float *alpha = sm.floats(kSmAlpha) + row0;
             if (key < kRows) {
                 const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
                 const float *alphas = reinterpret_cast<const float *>(p.at(p.s.alphas));
-                alpha[key] = mine ? __ldcg(alphas + row) : 0.f;
-                alpha[kGroupRows + key] = mine && p.s.kinds == 2u ? __ldcg(alphas + (uint64_t)p.s.octets * kOctet + row) : 0.f;
+                const float a = mine ? __ldcg(alphas + row) : 0.f;
+                const float b = mine && p.s.kinds == 2u ? __ldcg(alphas + (uint64_t)p.s.octets * kOctet + row) : 0.f;
+                // A query row that is not finite walks as zeros, so as not to make its octet's rows seek new
+                // references at every tile; the NaN is in its denominator.
+                const bool finite = a == a && b == b;
+                alpha[key] = finite ? a : 0.f;
+                alpha[kGroupRows + key] = finite ? b : 0.f;
+                if (!finite) row_sum = __uint_as_float(0x7fc00000u);
                 ref[key] = -kNoKey;
                 top[key] = top[kGroupRows + key] = INT32_MIN;
             } else if (key < kRows + kOctets) {
@@ -848,7 +855,6 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             }
         }
         if (!softmax_sync(sm, half, phase)) return;
-        float row_sum = 0.f;                                  // this warp's share of the denominator of row `lane`
         float row_ref = kNoKey;                               // reference of row `lane`, the same in every warp of the half
         float later = 1.f;                                    // what the row's sums are multiplied by at the next tile
         const uint32_t present = (1u << max(min(it.g.octets - (int32_t)(half * kOctets), (int32_t)kOctets), 0)) - 1u;
@@ -1012,7 +1018,8 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 // registers, and writes the same values; of the octets that are done again only.  Maxima left from
                 // earlier tiles do not lie above the reference they have led to and move nothing; nor does a NaN.
                 const float highest = __int_as_float(ordered(top[buf * kGroupRows + lane]));
-                if (((todo >> (lane >> 3)) & 1u) && highest > row_ref - 0.5f) {               // the margin covers the rounding of the maximum
+                // the margin covers the rounding of the maximum, and no more: a row does not move because another one does
+                if (((todo >> (lane >> 3)) & 1u) && highest > row_ref - fabsf(highest) * 0x1p-23f) {
                     const float down = exp2_approx(row_ref - (highest + kHeadroom));
                     row_ref = highest + kHeadroom;
                     ref[lane] = -row_ref;
@@ -1055,9 +1062,9 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
         if (!softmax_sync(sm, half, phase)) return;
         if (mine) {
             const uint64_t row = (uint64_t)it.g.first_octet * kOctet + row0 + key;
-            const float a = sm.floats(kSmAlpha)[row0 + key], m = row_ref;
-            // a NaN stands for a query row that is not finite, as do logits beyond FP32
-            const float l = a != a || m == INFINITY ? __uint_as_float(0x7fc00000u) : ((row_sum + sums[key]) + sums[kGroupRows + key]) + sums[2u * kGroupRows + key];
+            const float m = row_ref;
+            // logits beyond FP32 give NaN
+            const float l = m == INFINITY ? __uint_as_float(0x7fc00000u) : ((row_sum + sums[key]) + sums[kGroupRows + key]) + sums[2u * kGroupRows + key];
             if (it.whole()) {
                 const float sink = __ldg(reinterpret_cast<const float *>(p.a.sinks) + row % p.a.heads);
                 const float sink2 = sink * kLog2e, at = fmaxf(m, sink2), own = exp2_approx(m - at);

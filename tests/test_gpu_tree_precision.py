@@ -123,12 +123,13 @@ def peaked(rows, gap, *, ratio, noise, peak, period=0, seed=0):
 
 
 def repeated(made, times):
-    """The request `times` over: with more of them than SMs, most are worked on by one block from end to end."""
+    """The requests `times` over: with more of them than SMs, most are worked on by one block from end to end."""
     case, paths, cmp_paths, ori_scale, cmp_scale = made
     again = lambda t: None if t is None else t.repeat(times, *[1] * (t.ndim - 1))  # noqa: E731
-    n = len(case.q)
+    starts = case.cu_q[:-1] + len(case.q) * torch.arange(times, dtype=torch.int32)[:, None]
     case = replace(case, q=again(case.q), ori_block_table=again(case.ori_block_table), cmp_block_table=again(case.cmp_block_table),
-                   seq_lens=again(case.seq_lens), cu_q=torch.arange(0, times * n + 1, n, dtype=torch.int32), cmp_indices=again(case.cmp_indices))
+                   seq_lens=again(case.seq_lens), cu_q=torch.cat([starts.flatten(), torch.tensor([times * len(case.q)], dtype=torch.int32)]),
+                   cmp_indices=again(case.cmp_indices))
     return case, again(paths), again(cmp_paths), ori_scale, cmp_scale
 
 
@@ -172,3 +173,22 @@ def test_peaked_rows_as_the_decode_attention(rows, gap):
     mine_lse, theirs_lse = ((t.view(200, 3, 8) - want_lse).abs().max() for t in (lse, decode.lse.cpu().double()))
     print(f"rows {rows} gap {gap}: tree {float(mine):.5f} decode {float(theirs):.5f} lse {float(mine_lse):.6f} {float(theirs_lse):.6f}")
     assert mine <= math.sqrt(2) * theirs
+
+
+@pytest.mark.parametrize("ratio", [4, 128])
+def test_rows_that_are_not_finite_leave_the_others_alone(ratio):
+    """On walks of many tiles too, where references move: the other rows' results are those of a launch without them."""
+    made = make_tree_case([9, 40], [128 * 90, 128 * 70] if ratio == 128 else [9000, 7000], ratio=ratio, topk=1024, seed=12, spread=2.0)
+    case = made[0]
+    broken = replace(case, q=case.q.clone())
+    rows = [(0, 0), (3, 2), (20, 5), (48, 7)]
+    for i, (t, h) in enumerate(rows):
+        broken.q[t, h, 11 * i] = (math.nan, math.inf, -math.inf)[i % 3]
+    want, want_lse = launch(repeated(made, 30))
+    out, lse = launch(repeated((broken, *made[1:]), 30))
+    keep = torch.ones(49, 8, dtype=torch.bool)
+    for t, h in rows:
+        keep[t, h] = False
+    keep = keep.repeat(len(out) // 49, 1)
+    assert torch.equal(out[keep], want[keep]) and torch.equal(lse[keep], want_lse[keep])
+    assert out[~keep].isnan().all() and lse[~keep].isnan().all()
