@@ -1084,9 +1084,7 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
 
 // ------------------------------------------------------------------ walk: accumulate (warps 8-15)
 // Thread = channel of each 128-channel block, rows 32 h .. 32 h + 31: 128 running sums in registers.  The
-// integers of a block are read, joined and added while the tensor core fills the other block.  Sums are in
-// units of the current kind's channel scale: they change units where an item goes from one kind to the
-// other, and are scaled when they are stored.
+// integers of a block are read, joined, scaled and added while the tensor core fills the other block.
 __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
 {
     const uint32_t index = threadIdx.x - kWarpAccumulate * 32u, h = index >> 7, channel = index & 127u, warp = channel >> 5;
@@ -1111,15 +1109,7 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
         for (uint32_t j = it.begin; j < it.end; ++j, ++t) {
             const uint32_t buf = t & 1u, ph = (t >> 1) & 1u;
             if (!walk_wait<1>(sm, kBarWeightReady + buf, ph)) return;
-            if (j == (uint32_t)it.g.ori_tiles && j != it.begin) {
-#pragma unroll
-                for (int block = 0; block < 4; ++block) {
-                    const float units = __fdividef(__ldg(reinterpret_cast<const float *>(p.a.oriScale) + block * 128 + channel),
-                                                   __ldg(reinterpret_cast<const float *>(p.a.cmpScale) + block * 128 + channel));
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[block][r] = mul2(acc[block][r], pack2(units, units));
-                }
-            }
+            const float *scale = reinterpret_cast<const float *>(j < (uint32_t)it.g.ori_tiles ? p.a.oriScale : p.a.cmpScale) + channel;
             const uint32_t moved = sm.flags()[kFlagRescale + buf * 2u + h];
             if (moved) {
                 const ulonglong2 *factor = reinterpret_cast<const ulonglong2 *>(sm.ptr + kSmFactor) + buf * 16u + h * 8u;
@@ -1140,6 +1130,8 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
 #pragma unroll
             for (uint32_t block = 0; block < 4; ++block) {
                 const uint32_t half = block & 1u;
+                const float f = __ldg(scale + block * 128u);
+                const uint64_t f2 = pack2(f, f);
                 if (!walk_wait<1>(sm, kBarOutFull + half, (block >> 1) & 1u)) return;
                 tc_fence_after();
 #pragma unroll
@@ -1154,21 +1146,13 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     }
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i)
-                        acc[block][c * 4u + i] = add2(acc[block][c * 4u + i], pack2((float)((int32_t)hi[2 * i] * 256 + (int32_t)lo[2 * i]),
-                                                                                    (float)((int32_t)hi[2 * i + 1] * 256 + (int32_t)lo[2 * i + 1])));
+                        acc[block][c * 4u + i] = fma2(pack2((float)((int32_t)hi[2 * i] * 256 + (int32_t)lo[2 * i]),
+                                                            (float)((int32_t)hi[2 * i + 1] * 256 + (int32_t)lo[2 * i + 1])), f2, acc[block][c * 4u + i]);
                 }
             }
         }
         if (!walk_wait<1>(sm, kBarDone, items & 1u)) return;
         const uint32_t rows = (uint32_t)it.g.octets * kOctet;
-        const float *scale = reinterpret_cast<const float *>(it.end <= (uint32_t)it.g.ori_tiles ? p.a.oriScale : p.a.cmpScale) + channel;
-#pragma unroll
-        for (uint32_t block = 0; block < 4; ++block) {
-            const float f = __ldg(scale + block * 128u);
-            const uint64_t f2 = pack2(f, f);
-#pragma unroll
-            for (uint32_t r = 0; r < 16; ++r) acc[block][r] = mul2(acc[block][r], f2);
-        }
         auto value = [&](uint32_t block, uint32_t r) { return r & 1u ? high2(acc[block][r / 2u]) : low2(acc[block][r / 2u]); };
         if (it.whole()) {
             const float *inverse = sm.floats(kSmSum) + h * 32u;

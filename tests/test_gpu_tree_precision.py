@@ -9,7 +9,7 @@ import torch
 from npu_sparse_attn_sharedkv_int8 import PreparedAttention, PreparedTreeAttention
 from npu_sparse_attn_sharedkv_int8.reference import SharedKVCase
 from npu_sparse_attn_sharedkv_int8.tree_attention import path_masks
-from tests.tree_support import make_tree_case
+from tests.tree_support import check_dense, make_tree_case
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,19 @@ def test_rows_that_are_not_finite_leave_the_others_alone(ratio):
     keep = keep.repeat(len(out) // 49, 1)
     assert torch.equal(out[keep], want[keep]) and torch.equal(lse[keep], want_lse[keep])
     assert out[~keep].isnan().all() and lse[~keep].isnan().all()
+
+
+@pytest.mark.parametrize("ratio", [4, 128])
+def test_channels_without_a_scale(ratio):
+    """A channel may be zero, or next to it, in one cache and not in the other."""
+    case, paths, cmp_paths, ori_scale, cmp_scale = make_tree_case([9, 40], [128 * 90, 128 * 70] if ratio == 128 else [9000, 7000], ratio=ratio, topk=333,
+                                                                  seed=14)
+    cmp_scale[5], cmp_scale[140], cmp_scale[300], ori_scale[6], ori_scale[511] = 0, 0, 1e-36, 0, 1e-36
+    ori_scale[301] = cmp_scale[301] = 0
+    made = repeated((case, paths, cmp_paths, ori_scale, cmp_scale), 30)
+    out, lse = launch(made)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    dev = made[0].to("cuda")
+    worst = check_dense(dev, made[1].cuda(), None if cmp_paths is None else made[2].cuda(), ori_scale.cuda(), cmp_scale.cuda(), out.cuda(), lse.cuda())
+    assert worst[0] <= 1 and worst[1] <= 1, worst
+    assert out[..., 301].eq(0).all()
