@@ -208,3 +208,16 @@ def test_channels_without_a_scale(ratio):
     worst = check_dense(dev, made[1].cuda(), None if cmp_paths is None else made[2].cuda(), ori_scale.cuda(), cmp_scale.cuda(), out.cuda(), lse.cuda())
     assert worst[0] <= 1 and worst[1] <= 1, worst
     assert out[..., 301].eq(0).all()
+
+
+@pytest.mark.parametrize("options", [dict(counts=[64, 40, 64, 7], prefix=[128 * 2000, 128 * 900 + 77, 128 * 3000 + 5, 128 * 1500], ratio=128),
+                                     dict(counts=[30, 9], prefix=[14000, 5555], ratio=4, topk=777, spread=2.5),
+                                     dict(counts=[64, 31], prefix=[9000, 5000], window=4000, spread=1.5)], ids=["c128", "c4", "wide window"])
+def test_every_row_is_written(options):
+    """Long walks leave no element of a live row as it was (a NaN)."""
+    case, paths, cmp_paths, ori_scale, cmp_scale = make_tree_case(seed=100, **options)
+    move = lambda t: None if t is None else t.to("cuda")  # noqa: E731
+    tokens = len(case.q)
+    out, lse = (torch.full(shape, math.nan, dtype=dtype, device="cuda") for shape, dtype in (((tokens, 8, 512), torch.bfloat16), ((tokens, 8), torch.float32)))
+    PreparedTreeAttention(case.to("cuda"), move(paths), move(ori_scale), move(cmp_scale), cmp_paths=move(cmp_paths), output=out, lse_output=lse).run()
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
