@@ -161,8 +161,7 @@ int sharedkv_tree_attention(uint64_t args, int32_t device, void *stream)
 
 int sharedkv_tree_status(const void *workspace, void *stream)
 {
-    const int status = sharedkv::page_status(workspace, static_cast<cudaStream_t>(stream));
-    return status == SHAREDKV_ERANGE ? SHAREDKV_ETIMEDOUT : status;
+    return sharedkv::tree_status(workspace, static_cast<cudaStream_t>(stream));
 }
 
 uint32_t sharedkv_page_args_size(void) { return (uint32_t)sizeof(PagePoolArgs); }

@@ -59,6 +59,7 @@ int workspace_status(const void *workspace, cudaStream_t stream);
 // Drafted-tree attention (tree_attention.cu).
 uint64_t tree_workspace_bytes(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk);
 int tree_attention(const TreeAttentionArgs *args, cudaStream_t stream);
+int tree_status(const void *workspace, cudaStream_t stream);
 
 // Page pool (page_pool.cu).  `op` 0 resizes to `input`, 1 forks from the parents `input`.
 uint64_t page_workspace_bytes(uint32_t batch, uint32_t width);

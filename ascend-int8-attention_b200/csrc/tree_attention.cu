@@ -106,6 +106,9 @@ static_assert(sizeof(Group) == 32, "a descriptor is two 16-byte loads");
 // 256 bytes head (word 0 sticky status, word 1 arrivals of the union's blocks, words 2 and 3 the live tokens
 // and the tokens in front of the first request), cut points,
 // group descriptors and starts, query codes and alphas, union lists (ratio 4), partial results.
+// A launch writes all it reads, the arrivals included: it works on whatever bytes it finds.  Only the status outlives a
+// launch; it is a failure where it holds kTreeTimedOut, and nothing else.
+constexpr uint32_t kTreeTimedOut = 0x7472ee01u;
 struct TreeSpace {
     uint64_t cuts, groups, starts, codes, alphas, rows, counts, partials, bytes;
     uint32_t octets, slots, kinds;
@@ -272,10 +275,7 @@ __device__ bool last_block(const Tree &p, uint32_t blocks)
 {
     __shared__ uint32_t mine;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        mine = atomic_add_acq_rel(p.head() + 1, 1u);
-        if (mine + 1u == blocks) p.head()[1] = 0;             // as the next launch needs it
-    }
+    if (threadIdx.x == 0) mine = atomic_add_acq_rel(p.head() + 1, 1u);
     __syncthreads();
     return mine + 1u == blocks;
 }
@@ -337,7 +337,7 @@ __device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_
             finite ? unit : __uint_as_float(0x7fc00000u);
 }
 
-// Group descriptors of all slots, by one block; the head keeps the number of live tokens.
+// Group descriptors of all slots, by one block; the head gets the number of live tokens, and no arrivals yet.
 __device__ void describe_groups(const Tree &p)
 {
     __shared__ uint32_t shared_live;
@@ -345,7 +345,7 @@ __device__ void describe_groups(const Tree &p)
     const int32_t *cu = p.cu();
     const uint32_t live = live_requests(p, &shared_live);
     const uint32_t live_tokens = split::live_token_count(live ? cu[live] : 0, p.a.tokens);
-    if (threadIdx.x == 0) { p.head()[2] = live_tokens; p.head()[3] = live ? min((uint32_t)max(cu[0], 0), live_tokens) : 0u; }
+    if (threadIdx.x == 0) { p.head()[1] = 0; p.head()[2] = live_tokens; p.head()[3] = live ? min((uint32_t)max(cu[0], 0), live_tokens) : 0u; }
     for (uint32_t i = threadIdx.x; i < p.s.slots; i += blockDim.x) {
         uint32_t lo = 0, hi = live ? live - 1u : 0u;
         while (lo < hi) {
@@ -1239,7 +1239,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid
     if (flags[kFlagAbort]) {
         // A wait ran out: copies and products already issued may still land in this block's memory, so it
         // stays for far longer than they can take before it gives that memory up.
-        if (threadIdx.x == 0) p.head()[0] = kStatusWaitTimeout;
+        if (threadIdx.x == 0) p.head()[0] = kTreeTimedOut;
         for (uint32_t i = 0; i < 200u; ++i) __nanosleep(1000u);
         __syncthreads();
     }
@@ -1429,6 +1429,16 @@ int tree_launch_all(const TreeAttentionArgs &a, cudaStream_t stream, int sms)
 uint64_t tree_workspace_bytes(uint32_t tokens, uint32_t heads, uint32_t batch, uint32_t ratio, uint32_t topk)
 {
     return tree_space(tokens, heads, batch, ratio, topk).bytes;
+}
+
+int tree_status(const void *workspace, cudaStream_t stream)
+{
+    if (workspace == nullptr) return SHAREDKV_EINVAL;
+    uint32_t status = 0;
+    cudaError_t e = cudaMemcpyAsync(&status, workspace, sizeof(status), cudaMemcpyDeviceToHost, stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+    if (e != cudaSuccess) return (int)e;
+    return status == kTreeTimedOut ? SHAREDKV_ETIMEDOUT : SHAREDKV_OK;
 }
 
 int tree_attention(const TreeAttentionArgs *args, cudaStream_t stream)

@@ -96,9 +96,9 @@ class PreparedTreeAttention:
         self.workspace = allocate("tree_workspace", (max(need, 1024),), torch.uint8, device)
         _require(self.workspace.data_ptr() % 256 == 0, "Attention workspace must be 256-byte aligned")
         args.workspace = self.workspace.data_ptr()
-        # arrival counters and status start at zero and every launch leaves them so
-        with torch.cuda.device(device):
-            check(self.kernels.lib.sharedkv_workspace_init(args.workspace, current_stream(device.index)), "workspace init")
+        # Launches need no prepared workspace, so it does not matter which stream this runs on and when, or that a graph
+        # captures it: it only clears the status word, which recycled memory may hold.
+        self.workspace[:4].zero_()
         self.argument_address = ctypes.addressof(args)
         self._rebind_same_geometry(case, paths, cmp_paths=cmp_paths, output=out, lse_output=lse)
 

@@ -278,8 +278,9 @@ typedef struct TreeAttentionArgs {
     uint64_t sinks;      /* FP32 [heads]                                                 */
     uint64_t out;        /* BF16 [tokens, heads, 512]                                    */
     uint64_t lse;        /* FP32 [tokens, heads] or 0                                    */
-    uint64_t workspace;  /* >= sharedkv_tree_workspace_bytes(...) bytes, 256-aligned, prepared once by
-                            sharedkv_workspace_init; launches that can overlap need one each */
+    uint64_t workspace;  /* >= sharedkv_tree_workspace_bytes(...) bytes, 256-aligned, of any content (the
+                            status alone counts from when sharedkv_workspace_init, or a zero in the
+                            first word, has cleared it); launches that can overlap need one each */
     uint64_t oriStride, cmpStride;    /* bytes between pages, multiples of 16            */
     uint32_t tokens, heads, batch, oriTableWidth, cmpTableWidth, oriPages, cmpPages, ratio, window, topk;
     float softmaxScale;
@@ -291,7 +292,7 @@ SHAREDKV_API uint64_t sharedkv_tree_workspace_bytes(uint32_t tokens, uint32_t he
 SHAREDKV_API int launch_tree_attention(void *stream, const TreeAttentionArgs *args);
 SHAREDKV_API int sharedkv_tree_attention(uint64_t args, int32_t device, void *stream);
 /* Synchronises `stream`; SHAREDKV_OK, SHAREDKV_ETIMEDOUT (a wait inside a launch that used this workspace ran
- * out since it was prepared: that launch's results are invalid) or a cudaError_t. */
+ * out since its first word was cleared: that launch's results are invalid) or a cudaError_t. */
 SHAREDKV_API int sharedkv_tree_status(const void *workspace, void *stream);
 
 /* ------------------------------------------------------------------ page pool
