@@ -17,6 +17,7 @@ MAX_SEQUENCES = 8192
 _POINTERS = ("caches", "table", "lens", "refs", "workspace")
 _COUNTS = ("layers", "pages", "pageRows", "batch", "width", "reserved")
 _RESIZE, _FORK, _COPY, _KEEP = range(4)
+_REFUSED = -34                   # SHAREDKV_ERANGE
 
 
 class _Args(ctypes.Structure):
@@ -158,11 +159,19 @@ class PagePool:
             self._launch(_KEEP, address, kept.data_ptr(), width)
 
     def status(self):
-        """Synchronises the current stream; raises RuntimeError if a resize or fork of this pool was ever
-        refused on the device (its tables were then left as they were).  Diagnostic only."""
+        """Synchronises the current stream; raises RuntimeError if a resize or fork of this pool was
+        refused on the device (its tables were then left as they were), ever or since `clear_status`.
+        Diagnostic only."""
         with torch.cuda.device(self.device):
-            if self.kernels.lib.sharedkv_page_status(self.workspace.data_ptr(), current_stream(self.device.index)):
-                raise NativeError("A page pool operation was refused: too few free pages, a length beyond the block table or an unknown parent")
+            status = self.kernels.lib.sharedkv_page_status(self.workspace.data_ptr(), current_stream(self.device.index))
+        if status == _REFUSED:
+            raise NativeError("A page pool operation was refused: too few free pages, a length beyond the block table or an unknown parent")
+        check(status, "page pool status")
+
+    def clear_status(self):
+        """Forgets a refusal, in stream order: a server that has freed pages and tries again asks `status`
+        about the second attempt."""
+        self.workspace[:1].zero_()
 
 
 __all__ = ["MAX_KEPT", "MAX_SEQUENCES", "PagePool", "count_references"]

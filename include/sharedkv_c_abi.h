@@ -337,7 +337,8 @@ SHAREDKV_API int launch_page_keep(void *stream, const PagePoolArgs *args, const 
 /* Host-bridge forms: `op` 0 resize, 1 fork, 2 copy, 3 keep; `a`, `b` the device arrays, `n` the count. */
 SHAREDKV_API int sharedkv_page(uint64_t args, uint32_t op, uint64_t a, uint64_t b, uint32_t n, int32_t device, void *stream);
 /* Synchronises `stream`; SHAREDKV_OK, SHAREDKV_ERANGE (a resize or fork since the workspace was cleared
- * was refused on the device) or a cudaError_t. */
+ * was refused on the device) or a cudaError_t.  Between calls, sharedkv_workspace_init on the call's stream
+ * clears it again: a second attempt can be told from the first. */
 SHAREDKV_API int sharedkv_page_status(const void *workspace, void *stream);
 
 #ifdef __cplusplus

@@ -65,3 +65,35 @@ def test_keep_refuses_the_pools_own_lengths():
     with pytest.raises(ValueError, match="tensor of its own"):
         pool.keep(pool.lens, ints([[0], [0]]))
     pool.keep(pool.lens.clone(), ints([[0], [0]]))
+
+
+def test_a_refusal_can_be_handled():
+    """Too few pages; a sequence is freed; the second attempt holds and says so, also from a captured graph."""
+    cache = torch.randint(-127, 128, (6, 32, 1, 512), dtype=torch.int8, device="cuda")
+    table = torch.full((2, 6), -1, dtype=torch.int32, device="cuda")
+    pool = PagePool([cache], table, ints([0, 0]))
+    pool.resize(ints([96, 96]))
+    pool.status()
+    pool.resize(ints([128, 96]))
+    with pytest.raises(RuntimeError, match="refused"):
+        pool.status()
+    pool.clear_status()
+    pool.status()
+    pool.resize(ints([96, 0]))
+    pool.resize(ints([128, 0]))
+    pool.status()
+    assert pool.lens.tolist() == [128, 0] and pool.refs.sum() == 4
+    wanted = ints([128, 0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pool.clear_status()
+        pool.resize(wanted)
+    for lens, holds in (([128, 64], True), ([128, 96], False), ([192, 0], True)):
+        wanted.copy_(ints(lens))
+        graph.replay()
+        if holds:
+            pool.status()
+        else:
+            with pytest.raises(RuntimeError, match="refused"):
+                pool.status()
+    assert pool.lens.tolist() == [192, 0]
