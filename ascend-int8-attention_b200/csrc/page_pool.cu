@@ -500,7 +500,7 @@ int page_plan(uint32_t op, const PagePoolArgs *args, const int32_t *input, cudaS
     if (!caches_ok(a) || !table_ok(a) || !a.lens || !a.refs || !a.workspace || !input || a.lens % 4u || a.refs % 4u || a.workspace % 256u ||
         reinterpret_cast<uintptr_t>(input) % 4u)
         return SHAREDKV_EINVAL;
-    if (a.batch > kMaxSequences) return SHAREDKV_ERANGE;
+    if (a.batch > kMaxSequences || (uint64_t)a.batch * a.width > 0xffffffffull) return SHAREDKV_ERANGE;       // fresh pages are counted in 32 bits
     const int sms = device_sm_count();
     if (sms <= 0) return (int)cudaErrorInvalidDevice;
     Pool p = {};

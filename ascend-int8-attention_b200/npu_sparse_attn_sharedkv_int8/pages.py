@@ -67,6 +67,7 @@ class PagePool:
             _require(table.shape[1] * shape[1] < 2 ** 31, "The block table addresses too many rows")
         if lens is not None:
             _require(table.shape[0] <= MAX_SEQUENCES, f"A pool holds at most {MAX_SEQUENCES} sequences")
+            _require(table.numel() < 2 ** 32, "The block table has too many entries")
             self._check_sequences(lens, table, "lens")
             if refs is None:
                 refs = count_references(table, lens, shape[1], shape[0])

@@ -301,6 +301,7 @@ SHAREDKV_API int sharedkv_tree_status(const void *workspace, void *stream);
  * that share this page numbering.  A page is free when its count is zero; fresh pages are always the
  * lowest-numbered free ones, so results do not depend on timing.  Sequence b holds the pages
  * table[b, 0 .. ceil(lens[b] / pageRows) - 1]; the entries behind them are left as they were.
+ * resize and fork take at most 8192 sequences and a table of fewer than 2^32 entries.
  * Calls on one pool change it in place and must be ordered (one stream, or events).  resize and fork
  * do all of their work or none: with too few free pages, a length beyond the table or a parent
  * outside the batch the pool stays as it is and the status word (sticky, sharedkv_page_status) says
