@@ -1,5 +1,6 @@
 """Page-pool calls in the order a user makes them."""
 from pathlib import Path
+import random
 import re
 from types import SimpleNamespace
 
@@ -9,13 +10,10 @@ import torch
 from npu_sparse_attn_sharedkv_int8 import PagePool, PreparedTreeAttention
 from npu_sparse_attn_sharedkv_int8.reference import SharedKVCase
 from npu_sparse_attn_sharedkv_int8.tree_attention import path_masks
+from tests.test_gpu_pages import check, ints, make_pool
 from tests.tree_support import expected
 
 pytestmark = pytest.mark.gpu
-
-
-def ints(values):
-    return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
 def test_readme_example():
@@ -97,3 +95,22 @@ def test_a_refusal_can_be_handled():
             with pytest.raises(RuntimeError, match="refused"):
                 pool.status()
     assert pool.lens.tolist() == [192, 0]
+
+
+@pytest.mark.parametrize("batch, width, rows", [(8192, 3, 1), (8191, 4, 2), (4097, 9, 1), (2049, 40, 1)])
+def test_many_sequences(batch, width, rows):
+    """Up to the most that a pool holds, where a fork moves the table two columns at a time."""
+    rng = random.Random(batch)
+    pool, model = make_pool(rng, batch, batch * width + 100, layers=1, rows=rows, width=width, shared=True)
+    most = width * rows
+    for step in range(4):
+        if step % 2:
+            parents = [rng.randrange(-1, batch) for _ in range(batch)]
+            pool.fork(ints(parents))
+            model.fork(parents)
+        else:
+            wanted = [max(0, min(most, n + rng.randint(-2 * rows, 2 * rows))) for n in model.lens]
+            pool.resize(ints(wanted))
+            model.resize(wanted)
+        assert not model.refused
+        check(pool, model)
