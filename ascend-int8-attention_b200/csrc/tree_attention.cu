@@ -25,7 +25,8 @@
 // steps of 2^-12, they would all be lost: with one key 10 nats above 8192 others, 10 to 31 % of the output; so it is 0.2 to 0.3 %.)
 // The reference moves only when some logit exceeds it: the exact row maximum, a reduction over the 128 lanes
 // that hold the keys, is needed at those tiles alone.  It then stands three powers of two above the maximum
-// (kHeadroom), and one or two less from the next tile on if the row's weight in this tile is not spread over many keys.  So steps
+// (kHeadroom), one at an item's last tile, and one or two less from the next tile on if the row's weight in this tile is not
+// spread over many keys.  So steps
 // are 2^-14 of the largest weight where one key has most of it, as the decode attention's are, and 2^-12
 // where many keys share it and hide their rounding.  Always one power: 212 us for a C128 batch that takes 176 (every second
 // tile moves references), always three: 174.
@@ -1020,9 +1021,9 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                 const float highest = __int_as_float(ordered(top[buf * kGroupRows + lane]));
                 // the margin covers the rounding of the maximum, and no more: a row does not move because another one does
                 if (((todo >> (lane >> 3)) & 1u) && highest > row_ref - fabsf(highest) * 0x1p-23f) {
-                    const float down = exp2_approx(row_ref - (highest + kHeadroom));
-                    row_ref = highest + kHeadroom;
-                    ref[lane] = -row_ref;
+                    const float next = highest + (j + 1u < it.end ? kHeadroom : 1.f), down = exp2_approx(row_ref - next);
+                    row_ref = next;
+                    ref[lane] = -next;
                     factor *= down;
                     row_sum *= down;
                     moved = true;
