@@ -66,7 +66,7 @@ constexpr float kWeightSteps = 32638.f, kFine = 256.f;       // weight 1 in code
 constexpr uint32_t kCodeBias = 0x4b008000u;                  // bits of 2^23 + 128 * 256
 constexpr float kNoKey = -3.402823466e38f;                   // reference of a row that has met no key: the lowest finite value
 constexpr float kHeadroom = 3.f;                             // powers of two from a new maximum to the reference
-constexpr uint32_t kSpread = 22;                             // bits of a quarter in fine steps: twice the maximum, seen from the reference
+constexpr uint32_t kSpread = 21;                             // bits of an eighth in fine steps: the maximum, seen from the reference
 constexpr float kWideUnit = 0x1p-11f;                        // joined integers stay below 2^31
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kUnionRows = 1u << 18;                    // compressed rows a union bitmap covers at a time (32 KB)
@@ -1037,8 +1037,9 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
             mbar_arrive(sm.bar(kBarWeightReady + buf));
             row_sum = fmaf((float)(total - dithers), 1.f / kFine, row_sum);
             // Where a new maximum leaves little weight for others, the reference may be close to it from the next tile on:
-            // where the second heaviest of the tile's four runs of 32 keys weighs less than twice the maximum.  Not for the
-            // sake of one last tile (44.3 against 44.8 us on the window batch).
+            // where the second heaviest of the tile's four runs of 32 keys weighs less than the maximum.  (With twice and half the
+            // maximum the C4 batch takes 79 and 78 us against 77.5, and errors are the same to 1e-4 up to half.)  Not for the sake
+            // of one last tile (44.3 against 44.8 us on the window batch).
             if (todo && j + 2u < it.end) {
                 uint8_t *spread = reinterpret_cast<uint8_t *>(sm.ptr + kSmSpread) + (row0 + lane) * 4u;
                 spread[warp] = (uint8_t)(32 - __clz((int32_t)(total - dithers)));
