@@ -26,7 +26,7 @@ def launch(made):
 def definition(made):
     """(out, lse) of the live tokens of request 0 in float64."""
     case, paths, cmp_paths, ori_scale, cmp_scale = made
-    case, ori_scale, cmp_scale = case.to("cuda"), ori_scale.cuda(), cmp_scale.cuda()
+    case, ori_scale, cmp_scale = case.to("cuda"), ori_scale.cuda(), None if cmp_scale is None else cmp_scale.cuda()
     n = int(case.cu_q[1])
     prefix = int(case.seq_lens[0]) - n
     whole = prefix // case.ratio
@@ -221,3 +221,28 @@ def test_every_row_is_written(options):
     out, lse = (torch.full(shape, math.nan, dtype=dtype, device="cuda") for shape, dtype in (((tokens, 8, 512), torch.bfloat16), ((tokens, 8), torch.float32)))
     PreparedTreeAttention(case.to("cuda"), move(paths), move(ori_scale), move(cmp_scale), cmp_paths=move(cmp_paths), output=out, lse_output=lse).run()
     assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("options", [dict(prefix=[5000], window=4000), dict(prefix=[9000], ratio=4, topk=1024), dict(prefix=[128 * 2500 + 3], ratio=128)],
+                         ids=["wide window", "c4", "c128"])
+def test_uneven_rows(options, seed):
+    """Rows that range from flat to a single key, side by side in their octets, with keys that stand out in every part of the walk.
+    A row's error: BF16's half step, and the codes' of up to 4096 keys, sqrt(n) / 2 steps of 8 / 32638 of the largest weight at
+    the very most (0.008 of the largest row, where the sum of a row's weighted values may be as small as that)."""
+    made = make_tree_case([24], seed=seed, **options)
+    case, gen = made[0], torch.Generator().manual_seed(seed + 50)
+    case.q = (case.q.float() * torch.exp(torch.randn(24, 8, 1, generator=gen) * 0.8)).to(torch.bfloat16)
+    for cache in (case.ori, case.cmp) if case.ratio > 1 else (case.ori,):
+        rows = cache.view(-1, 512)
+        for r in torch.randint(0, len(rows), (30,), generator=gen).tolist():
+            t, h = int(torch.randint(0, 24, (1,), generator=gen)), int(torch.randint(0, 8, (1,), generator=gen))
+            toward = case.q[t, h].float()
+            rows[r] = (rows[r].float() * 0.7 + toward / toward.norm() * 22 * (10 + 30 * float(torch.rand(1, generator=gen)))).round().clamp(-127, 127).to(torch.int8)
+    want, want_lse = definition(made)
+    copies = 40
+    out, lse = launch(repeated(made, copies))
+    errors = row_errors(out.view(copies, 24, 8, 512), want)
+    print(f"{options} seed {seed}: out {float(errors.max()):.5f} mean {float(errors.mean()):.5f} lse {float((lse.view(copies, 24, 8) - want_lse).abs().max()):.5f}")
+    assert errors.max() <= 0.012 and errors.square().mean().sqrt() <= 0.003
+    assert ((lse.view(copies, 24, 8) - want_lse).abs() <= 2.0 ** -9 + want_lse.abs() * 2.0 ** -12).all()
