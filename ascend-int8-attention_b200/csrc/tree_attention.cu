@@ -60,7 +60,7 @@ constexpr uint32_t kEncodeThreads = 256, kUnionThreads = 1024, kMergeThreads = 2
 constexpr uint32_t kWarpAccumulate = 8, kWarpIssue = 16, kWarpProduce = 18, kProducers = 2;
 // Registers: launched with 96 per thread; accumulate (two warps of every SM partition) grows to hold
 // 128 running sums a thread, the others shrink.
-constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 64, kRegsAccumulate = 152, kRegsIssue = 48;
+constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 72, kRegsAccumulate = 144, kRegsIssue = 48;
 static_assert(2 * kRegsSoftmax + 2 * kRegsAccumulate + kRegsIssue <= 5 * kRegsLaunch, "register shares exceed the launch allocation");
 constexpr float kWeightSteps = 32638.f, kFine = 256.f;       // weight 1 in codes (the largest is 127 * 256 + 127), and a code in fine steps
 constexpr uint32_t kCodeBias = 0x4b008000u;                  // bits of 2^23 + 128 * 256
@@ -1009,10 +1009,11 @@ __device__ void softmax(const Tree &p, const WalkShared &sm, uint32_t tmem)
                     flags[vote == zero + 2u ? zero : vote + 1u] = 0;
                     flags[kFlagRescale + buf * 2u + half] = todo | (low & 0xffu ? 1u : 0u) | (low & 0xff00u ? 2u : 0u) | (low & 0xff0000u ? 4u : 0u) | (low >> 24 ? 8u : 0u);
                 }
+                if (!(todo | low)) break;
                 float factor = later;
                 later = 1.f;
                 if (!todo) {
-                    if (low && warp == 0) sm.floats(kSmFactor)[buf * kGroupRows + row0 + lane] = factor;
+                    if (warp == 0) sm.floats(kSmFactor)[buf * kGroupRows + row0 + lane] = factor;
                     break;
                 }
                 // Every warp works out the new references by itself, from the maxima and the old ones in its
@@ -1132,9 +1133,9 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
 #pragma unroll
             for (uint32_t block = 0; block < 4; ++block) {
                 const uint32_t half = block & 1u;
+                if (!walk_wait<1>(sm, kBarOutFull + half, (block >> 1) & 1u)) return;
                 const float f = __ldg(scale + block * 128u);
                 const uint64_t f2 = pack2(f, f);
-                if (!walk_wait<1>(sm, kBarOutFull + half, (block >> 1) & 1u)) return;
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t c = 0; c < 4; ++c) {
