@@ -59,7 +59,7 @@ constexpr uint32_t kWalkThreads = 640;
 constexpr uint32_t kEncodeThreads = 256, kUnionThreads = 1024, kMergeThreads = 256;
 constexpr uint32_t kWarpAccumulate = 8, kWarpIssue = 16, kWarpProduce = 18, kProducers = 2;
 // Registers: launched with 96 per thread; accumulate (two warps of every SM partition) grows to hold
-// 128 running sums a thread, the others shrink.
+// 128 running sums a thread, the others shrink.  (64 / 152 / 48: C128 batch 177 us against 174.)
 constexpr uint32_t kRegsLaunch = 96, kRegsSoftmax = 72, kRegsAccumulate = 144, kRegsIssue = 48;
 static_assert(2 * kRegsSoftmax + 2 * kRegsAccumulate + kRegsIssue <= 5 * kRegsLaunch, "register shares exceed the launch allocation");
 constexpr float kWeightSteps = 32638.f, kFine = 256.f;       // weight 1 in codes (the largest is 127 * 256 + 127), and a code in fine steps
@@ -286,7 +286,7 @@ __device__ bool last_block(const Tree &p, uint32_t blocks)
 // row.  Codes go out as the walk's B operand wants them: [kind][segment][plane][octet] blocks of 8 rows x
 // 128 bytes, swizzled, so that a group's rows of a plane are one contiguous copy.  160 instructions a row and
 // kind, packed FP32 where it can be, against 8 KB read and 8 KB per kind written an octet: 4096 octets of a
-// ratio-128 layer take 21 us (4.7 TB/s, two thirds of the issue slots).
+// ratio-128 layer take 22 us (4.5 TB/s, two thirds of the issue slots).
 __device__ __forceinline__ void encode_row(const Tree &p, uint32_t kind, uint32_t octet, uint32_t row, const uint64_t (&q)[8], const float *sm_scale)
 {
     const uint32_t lane = threadIdx.x & 31u;
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kEncodeThreads) tree_encode_kernel(const __gri
 // One block per group.  Rows are ranked by the bits before theirs in a bitmap, so the list ascends whatever
 // order the atomics ran in.  An entry carries its location (page * 32 + row in page, -1 when the page
 // is missing) and, per octet, how often the octet's token names it.  A chain of some twelve dependent steps between
-// barriers, so bound by latency: 64 groups of eight lists of 1024 take 13 us.
+// barriers, so bound by latency: 64 groups of eight lists of 1024 take 13 us behind the encode kernel, 16 alone.
 __global__ void __launch_bounds__(kUnionThreads, 1) tree_union_kernel(const __grid_constant__ Tree p)
 {
     extern __shared__ uint32_t smem[];
@@ -1180,8 +1180,8 @@ __device__ void accumulate(const Tree &p, const WalkShared &sm, uint32_t tmem)
     }
 }
 
-// 7528 tiles of a C128 batch (101 GFLOP) take 155 us on 148 SMs, 51 tiles a block: the tensor pipe is active for 44 % of
-// it.  A tile without a new reference takes the softmax warps 3750 cycles (2140 of them for the weights), which is what
+// 7528 tiles of a C128 batch (101 GFLOP) take 164 us on 148 SMs, 51 tiles a block: the tensor pipe is active for 41 % of
+// it.  A tile without a new reference takes the softmax warps 4100 cycles (over half of them for the weights), which is what
 // bounds the walk; the life of a tile, from its fetch into one of two places to its last product, takes
 // nearly twice that.  Tiles are 128 keys because the INT8 MMA is full at M = 128, and groups 64 rows because N = 128
 // balances its operand reads with its arithmetic (64 cycles; N = 64 takes 48) and 64 KB of codes are what fits beside two tiles.
@@ -1253,7 +1253,7 @@ __global__ void __launch_bounds__(kWalkThreads, 1) tree_walk_kernel(const __grid
 }
 
 // ------------------------------------------------------------------ merge
-// 147 cuts on 148 SMs leave up to 147 groups of two pieces or more, 128 KB each: 10 us, the chain cut -> data ->
+// 147 cuts on 148 SMs leave up to 147 groups of two pieces or more, 128 KB each: 9 to 10 us, the chain cut -> data ->
 // output and two waves of blocks.  Block (i, o): octet o of the group that cut i is the first to fall into.  Pieces are joined in piece
 // order: M = max of the references and the sink, out = sum O 2^(ref - M) / (sum l 2^(ref - M) + sink).
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const __grid_constant__ Tree p)
@@ -1400,9 +1400,9 @@ int tree_launch_all(const TreeAttentionArgs &a, cudaStream_t stream, int sms)
     p.a = a;
     p.s = tree_space(a.tokens, a.heads, a.batch, a.ratio, a.topk);
     p.grid = (uint32_t)sms < split::kMaxCtas ? (uint32_t)sms : split::kMaxCtas;
-    // A window layer's groups of two or three tiles stay whole and need no merge kernel: 13.0 against 15.6 us for one
-    // request of 8 tokens (whose two tiles could run side by side), 43.5 against 45.2 us for 48 of 1 to 63 with 16 heads,
-    // 15.3 against 17.0 us for four requests and a window of 200 rows.
+    // A window layer's groups of two or three tiles stay whole and need no merge kernel: 16.9 against 17.8 us for one
+    // request of 8 tokens (whose two tiles could run side by side), 44.2 against 46.0 us for 48 of 1 to 63 with 16 heads,
+    // 16.9 against 17.9 us for four requests and a window of 200 rows.
     const uint32_t window_tiles = (a.window + kTreeDraft + kTreePage - 2u) / kTile + 1u;
     p.splits = a.ratio != 1u || window_tiles > kWholeTiles;
     const bool listed = a.ratio == 4u;
